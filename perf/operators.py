@@ -4,7 +4,8 @@
 
 ``run`` computes a case in its plain form (elementary torch operations in 32 bits) or, where ``own`` is true, with the calls a
 user makes.  Microscaled operands are the layout the framework documents: codes uint8 [rows, Kp / 2] (E2M1, element 2i in the low
-nibble) or [rows, Kp] (E4M3), scales uint8 [rows, Kp / 32] (E8M0), Kp = K rounded up to a multiple of 128, zero codes behind K.
+nibble) or [rows, Kp] (E4M3), scales uint8 [Kp / 128, rows, 4] (E8M0, the scale of block b of row r at [b / 4, r, b % 4]), Kp = K
+rounded up to a multiple of 256, zero codes behind K.
 """
 import math
 
@@ -20,8 +21,8 @@ E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 EPS = 1e-6
 
 
-def pad128(k):
-    return -(-k // 128) * 128
+def padded(k):
+    return -(-k // 256) * 256
 
 
 # ---------------------------------------------------------------------------------------------------------------- cases
@@ -73,7 +74,7 @@ def draw(rng):
     if op == "gemm":
         rows, cols, width = _log(rng, 1, 32768), _log(rng, 16, 8192), _log(rng, 32, 8192)
         if rng.random() < 0.5:
-            cols, width = -(-cols // 128) * 128, pad128(width)
+            cols, width = -(-cols // 128) * 128, padded(width)
         rows = min(rows, max(1, 21320 * 4096 * 4096 // (2 * cols * width)), max(1, 21320 * 4096 // (2 * cols)))
         out = rng.choice(("f16", "bf16", "f32"))
         return dict(op=op, rows=rows, cols=cols, width=width, a=rng.choice(("fp8", "fp4")), bias=rng.random() < 0.7,
@@ -160,9 +161,9 @@ def prepare(case, seed):
 
 # ---------------------------------------------------------------------------------------------------------- plain forms
 def _mx_blocks(x, fmt):
-    """(|x|-scaled and rounded values [m, blocks, 32] in units of the scale, exponents [m, blocks]) of fp32 rows, padded."""
+    """(rounded values in units of their scale [m, blocks, 32], exponents [m, blocks]) of fp32 rows, padded."""
     m, k = x.shape
-    b = torch.zeros(m, pad128(k), dtype=torch.float32, device=x.device)
+    b = torch.zeros(m, padded(k), dtype=torch.float32, device=x.device)
     b[:, :k] = x
     b = b.view(m, -1, 32)
     amax = b.abs().amax(2)
@@ -180,10 +181,15 @@ def _mx_blocks(x, fmt):
     return torch.copysign(r, v), e
 
 
+def _mx_scales(e):
+    """E8M0 bytes of exponents [m, blocks], in the operand's order."""
+    return (e + 127).to(torch.uint8).view(e.shape[0], -1, 4).transpose(0, 1).contiguous()
+
+
 def _mx_pack(x, fmt):
     """(codes, scales) of fp32 rows."""
     v, e = _mx_blocks(x, fmt)
-    scales = (e + 127).to(torch.uint8)
+    scales = _mx_scales(e)
     if fmt == "fp8":
         return v.view(x.shape[0], -1).to(torch.float8_e4m3fn).view(torch.uint8), scales
     a = v.abs()
@@ -200,13 +206,14 @@ def _mx_values(codes, scales, fmt):
         table = torch.tensor(E2M1 + tuple(-x for x in E2M1), device=codes.device)
         v = torch.stack((table[(codes & 15).long()], table[(codes >> 4).long()]), 2)
     v = v.view(codes.shape[0], -1, 32)
-    return (v * torch.exp2(scales.float() - 127)[..., None]).view(codes.shape[0], -1)
+    e = scales.float().transpose(0, 1).reshape(codes.shape[0], -1) - 127
+    return (v * torch.exp2(e)[..., None]).view(codes.shape[0], -1)
 
 
 def _mx_out(x, fmt):
     """What a quantising call hands back: 8-bit codes as they are, 4-bit ones as the values they stand for."""
     v, e = _mx_blocks(x, fmt)
-    scales = (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+    scales = _mx_scales(e).view(torch.float8_e8m0fnu)
     if fmt == "fp8":
         return {"codes": v.view(x.shape[0], -1).to(torch.float8_e4m3fn), "scales": scales}
     return {"values": (v * torch.exp2(e.float())[..., None]).view(x.shape[0], -1)[:, :x.shape[1]].to(torch.bfloat16), "scales": scales}
@@ -305,15 +312,15 @@ def _exact_round(v, fmt):
 
 def _exact_mx(y, fmt):
     m, k = y.shape
-    b = torch.nn.functional.pad(y, (0, pad128(k) - k)).view(m, -1, 32)
+    b = torch.nn.functional.pad(y, (0, padded(k) - k)).view(m, -1, 32)
     amax = b.abs().amax(2)
     e = torch.floor(torch.log2(amax)) - EMAX[fmt]
     e = torch.where(torch.exp2(e + EMAX[fmt]) > amax, e - 1, torch.where(torch.exp2(e + EMAX[fmt] + 1) <= amax, e + 1, e))
     e = torch.where(amax < 2.0 ** -126, torch.full_like(e, -127), e.clamp(-127, 127))
     c = _exact_round(b / torch.exp2(e)[..., None], fmt)
     if fmt == "fp8":
-        return {"codes": c.view(m, -1), "scales": torch.exp2(e)}
-    return {"values": (c * torch.exp2(e)[..., None]).view(m, -1)[:, :k], "scales": torch.exp2(e)}
+        return {"codes": c.view(m, -1), "scales": torch.exp2(e).view(m, -1, 4).transpose(0, 1)}
+    return {"values": (c * torch.exp2(e)[..., None]).view(m, -1)[:, :k], "scales": torch.exp2(e).view(m, -1, 4).transpose(0, 1)}
 
 
 def _exact_values(codes, scales, fmt):
@@ -326,7 +333,7 @@ def _exact_values(codes, scales, fmt):
         sign, e, f = v >> 7, (v >> 3) & 15, (v & 7).double() / 8
         bias = 7
     a = torch.where(e > 0, (1 + f) * torch.exp2((e - bias).double()), f * 2.0 ** (1 - bias))
-    return torch.where(sign > 0, -a, a) * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+    return torch.where(sign > 0, -a, a) * torch.exp2(scales.double() - 127).permute(1, 0, 2).flatten(1).repeat_interleave(32, 1)
 
 
 def exact(case, seed):
@@ -369,11 +376,11 @@ def exact(case, seed):
 
 # ----------------------------------------------------------------------------------------------------------------- work
 def _mx_bytes(m, k, fmt):
-    return m * pad128(k) * BYTES[fmt] + m * pad128(k) / 32
+    return m * padded(k) * BYTES[fmt] + m * padded(k) / 32
 
 
 def _mx_out_bytes(m, k, fmt):
-    return _mx_bytes(m, k, fmt) if fmt == "fp8" else m * k * 2 + m * pad128(k) / 32
+    return _mx_bytes(m, k, fmt) if fmt == "fp8" else m * k * 2 + m * padded(k) / 32
 
 
 def work(case):
