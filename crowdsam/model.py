@@ -77,7 +77,7 @@ def profile(on=True, ranges=True):
         trace.enable()
     else:
         trace.disable()
-_WORK_STREAM = True          # generate() on its own high-priority stream (False: the caller's stream; tests toggle it)
+_WORK_STREAM = True          # generate() on its own stream (False: the caller's stream; tests toggle it)
 _WINDOWED_REGIONS = True      # small-region clean-up and RLE inside the masks' boxes (False: whole frames)
 
 
@@ -242,7 +242,7 @@ class CrowdSAM:
             # implicit synchronisation with every blocking stream costs the pipelined modes 1.3 ms per frame
             # (profiles/r04_eps_pipeline_overlap.txt).  Callers on other streams are ordered before / after it.
             if self._work_stream is None:
-                self._work_stream = torch.cuda.Stream(device=self.device, priority=-1)
+                self._work_stream = torch.cuda.Stream(device=self.device)
             cur = torch.cuda.current_stream(self.device)
             if cur == self._work_stream:
                 return self._generate_masks(image)
@@ -569,16 +569,16 @@ class CrowdSAM:
         n_batches = 0
         batch_size = self.points_per_batch
         # With the next frame's encoders running beside it (early prefetch), the EPS sweep -- a chain of ~60 short kernels per
-        # batch, each waiting for the one before -- goes onto a HIGH-priority stream: its workgroups are dispatched ahead of the
-        # encoder GEMMs' whenever a CU frees up, so the chain's latency stays close to what it is on an idle GPU
+        # batch, each waiting for the one before -- goes onto a stream of its own.  Every stream keeps the default priority:
+        # streams of different priorities have been seen to stop for good on this part.
         sweep_ctx = contextlib.ExitStack()
         if early and self._work_stream is not None and torch.cuda.current_stream() == self._work_stream:
-            early_hi = False                        # the frame's own stream already has the high priority
+            early_hi = False                        # the frame has its own stream already
         else:
             early_hi = early
         if early_hi:
             if self._hi_stream is None:
-                self._hi_stream = torch.cuda.Stream(device=dev, priority=-1)
+                self._hi_stream = torch.cuda.Stream(device=dev)
             self._hi_stream.wait_stream(torch.cuda.current_stream())
             main_stream = torch.cuda.current_stream()
             sweep_ctx.enter_context(torch.cuda.stream(self._hi_stream))

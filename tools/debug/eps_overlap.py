@@ -76,7 +76,7 @@ for mode in modes:
     m.generate(frames[0], next_image=frames[0]); m.generate(frames[0])
     torch.cuda.synchronize()
     t0 = time.perf_counter()
-    work = torch.cuda.Stream(priority=-1) if os.environ.get("WORK_STREAM") == "1" else torch.cuda.current_stream()
+    work = torch.cuda.Stream() if os.environ.get("WORK_STREAM") == "1" else torch.cuda.current_stream()
     with torch.cuda.stream(work):
         if mode == "serial":
             for f in frames[2:]:
