@@ -1,0 +1,134 @@
+// Shared pieces of the microscaled (MX) operators and of the row operators that take bfloat16 beside fp16 / fp32.
+//
+// An MX operand of R rows and K columns (include/csam.h has the layout users see):
+//   codes   [R][Kp / 2] (E2M1, element 2i in the low nibble) or [R][Kp] (E4M3), Kp = K rounded up to 256, zero codes behind K;
+//   scales  [Kp / 128][R][4] E8M0 bytes: block b (32 elements) of row r at [b / 4][r][b % 4].  The four scales of a 128-wide step
+//           of neighbouring rows lie side by side, so a wave fetches the scales of 32 or 64 rows as one run of whole cache lines;
+//           row-major bytes would cost a 128-byte line per row and step.
+#pragma once
+#include "csam_common.h"
+
+#define CSAM_DT_BF16 2
+#define CSAM_MX_FP4 0
+#define CSAM_MX_FP8 1
+
+typedef __bf16 bf16_t;
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float csam_lo_bf16(unsigned u) { return __builtin_bit_cast(float, u << 16); }
+__device__ __forceinline__ float csam_hi_bf16(unsigned u) { return __builtin_bit_cast(float, u & 0xffff0000u); }
+template <typename T> __device__ __forceinline__ float csam_to_f32(T v) { return (float)v; }
+
+// 8 consecutive elements as fp32.  VEC: 16-byte aligned, all eight inside; otherwise `n` (<= 8, may be <= 0) of them, zeros behind.
+template <typename T>
+__device__ __forceinline__ void csam_load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const floatx4 a = *(const floatx4*)p, b = *(const floatx4*)(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+  } else if constexpr (__is_same(T, half_t)) {
+    const half8_t h = *(const half8_t*)p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+  } else {
+    const uintx4 u = *(const uintx4*)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = csam_lo_bf16(u[i]), v[2 * i + 1] = csam_hi_bf16(u[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void csam_load8_tail(const T* p, int n, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+}
+// 8 consecutive elements, rounded to nearest even
+template <typename T>
+__device__ __forceinline__ void csam_store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *(floatx4*)p = floatx4{v[0], v[1], v[2], v[3]};
+    *(floatx4*)(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
+  } else {
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    vec8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (T)v[i];
+    *(vec8*)p = h;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void csam_store8_tail(T* p, int n, const float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = (T)v[i];
+}
+
+// value of an E8M0 byte: 2^(s - 127); 255 is NaN, 0 the subnormal 2^-127
+__device__ __forceinline__ float csam_e8m0(unsigned s) {
+  const unsigned bits = s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23;
+  return __builtin_bit_cast(float, bits);
+}
+
+// value of lane ^ 1 / ^ 2 within a quad, and the lane 4 / 8 further round within 16
+template <int CTRL>
+__device__ __forceinline__ unsigned csam_dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+
+// Quantises the 8 values of this lane, whose quad of lanes holds one block of 32: returns the block's E8M0 byte and the codes
+// (E2M1: 32 bits in c[0]; E4M3: 64 bits).
+//   byte = max(exponent(amax) - emax, 0) on the biased fp32 exponent = floor(log2 amax) - emax + 127; a subnormal or zero amax has
+//   exponent field 0, so its byte is 0; NaN and infinity have 255 -> byte 255 (every value of the block reads as NaN), codes 0.
+// amax is an integer maximum of the magnitudes' bits: fmaxf would drop a NaN.  x / 2^(byte-127) is exact in fp32 (a power of two; the
+// only results that could be subnormal come from elements 2^-100 below the block's largest, which round to zero in either format),
+// so the one rounding is the converter's to E2M1 / E4M3, ties to even; both saturate (E4M3 by the clamp: the converter's own overflow
+// would give NaN).
+template <int FMT>
+__device__ __forceinline__ unsigned csam_mx_quant8(const float (&v)[8], unsigned (&c)[2]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu);
+  m = max(m, csam_dpp<0xB1>(m));                          // quad_perm 1,0,3,2
+  m = max(m, csam_dpp<0x4E>(m));                          // quad_perm 2,3,0,1
+  const unsigned e = m >> 23;
+  constexpr unsigned EMAX = FMT == CSAM_MX_FP4 ? 2 : 8;
+  const unsigned byte = e == 255u ? 255u : e > EMAX ? e - EMAX : 0u;
+  if constexpr (FMT == CSAM_MX_FP4) {
+    const float scale = __builtin_bit_cast(float, byte == 0u ? 0x00400000u : byte << 23);
+    unsigned q = 0;
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], scale, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], scale, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[4], v[5], scale, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
+    c[0] = e == 255u ? 0u : q;
+    c[1] = 0u;
+  } else {
+    const float inv = __builtin_bit_cast(float, (254u - (byte > 253u ? 253u : byte)) << 23);
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -448.f, 448.f);
+    int a = 0, b = 0;
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], a, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], a, true);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(w[4], w[5], b, false);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(w[6], w[7], b, true);
+    c[0] = e == 255u ? 0u : (unsigned)a;
+    c[1] = e == 255u ? 0u : (unsigned)b;
+  }
+  return byte;
+}
+
+// Codes and scales of chunk `c8` (8 elements) of row `row`; 16 consecutive lanes hold a 128-wide group, so the four block bytes are
+// put together with two rotations within 16 lanes and leave as one dword.
+template <int FMT>
+__device__ __forceinline__ void csam_mx_store8(const float (&v)[8], uint8_t* codes, long ldc, uint8_t* scales, long sstride, long row,
+                                               int c8) {
+  unsigned c[2];
+  unsigned s = csam_mx_quant8<FMT>(v, c) << (8 * ((c8 >> 2) & 3));
+  s |= csam_dpp<0x124>(s);                                // row_ror:4
+  s |= csam_dpp<0x128>(s);                                // row_ror:8
+  if constexpr (FMT == CSAM_MX_FP4) *(unsigned*)(codes + row * ldc + c8 * 4) = c[0];
+  else *(uintx2*)(codes + row * ldc + c8 * 8) = uintx2{c[0], c[1]};
+  if ((c8 & 15) == 0) *(unsigned*)(scales + (long)(c8 >> 4) * sstride + row * 4) = s;
+}

@@ -1,0 +1,305 @@
+// Quantisation to and from microscaled (MX) operands, and the root-mean-square norm that can hand its rows out as one.
+// All of it is bound by memory: a pass reads each input once and writes each output once.
+#include <type_traits>
+#include "mx_common.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------- quantise
+// A workgroup takes 32 rows x 256 columns: 512 bytes (16-bit inputs) of a row per half-wave, and a scale dword of 32 neighbouring
+// rows per 128 columns, i.e. a whole 128-byte line of scales per workgroup and group (no line is shared between XCDs).
+constexpr int Q_ROWS = 32, Q_COLS = 256;
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, long ldx, uint8_t* __restrict__ codes, long ldc,
+                                                          uint8_t* __restrict__ scales, long sstride, int M, int K, int nseg, int vec) {
+  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * Q_ROWS + (threadIdx.x >> 5);
+  const int c8 = seg * (Q_COLS / 8) + (threadIdx.x & 31), k = c8 * 8;
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 8 * i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    if (row < M && k < K) {
+      if (vec && k + 8 <= K) csam_load8(x + (long)row * ldx + k, v[i]);
+      else csam_load8_tail(x + (long)row * ldx + k, K - k, v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 8 * i;
+    if (row < M) csam_mx_store8<FMT>(v[i], codes, ldc, scales, sstride, row, c8);       // whole half-waves share a row
+  }
+}
+
+template <int FMT>
+__device__ __forceinline__ void mx_values8(const uint8_t* codes, float scale, float (&v)[8]) {
+  if constexpr (FMT == CSAM_MX_FP4) {
+    const unsigned q = *(const unsigned*)codes;
+    const float2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+    const float2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+    const float w[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = w[i] * scale;
+  } else {
+    const uintx2 q = *(const uintx2*)codes;
+    const float2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(q[0], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q[0], true);
+    const float2_t c = __builtin_amdgcn_cvt_pk_f32_fp8(q[1], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(q[1], true);
+    const float w[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = w[i] * scale;
+  }
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes, long ldc, const uint8_t* __restrict__ scales,
+                                                            long sstride, T* __restrict__ y, long ldy, int M, int K, int nseg, int vec) {
+  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * Q_ROWS + (threadIdx.x >> 5);
+  const int c8 = seg * (Q_COLS / 8) + (threadIdx.x & 31), k = c8 * 8;
+  if (k >= K) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 8 * i;
+    if (row >= M) continue;
+    const unsigned s = scales[(long)(c8 >> 4) * sstride + (long)row * 4 + ((c8 >> 2) & 3)];
+    float v[8];
+    mx_values8<FMT>(codes + row * ldc + (long)c8 * (FMT == CSAM_MX_FP4 ? 4 : 8), csam_e8m0(s), v);
+    if (vec && k + 8 <= K) csam_store8(y + (long)row * ldy + k, v);
+    else csam_store8_tail(y + (long)row * ldy + k, K - k, v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- RMS norm
+// h = x + r, y = h * rsqrt(mean(h^2) + eps) * gamma: the row stays in registers between the sum and the scaling (one read of x and
+// r, one write of h and y).  NW waves share a row of up to NW * MAXC * 512 columns; NW = 1 needs no barrier.  h is summed and scaled in
+// fp32 before it is rounded to r's type.
+struct RmsArgs {
+  const void* x; long ldx;
+  const void* r; long ldr;
+  void* h; long ldh;
+  const float* gamma;
+  float eps;
+  void* y; long ldy; int y_kind;          // CSAM_DT_*, or RMS_MX + CSAM_MX_*
+  uint8_t* scales; long sstride;
+  int M, D, Dp, vec, rows;                // rows: rows of a row slot (a wave when NW = 1, the workgroup otherwise)
+};
+constexpr int RMS_MX = 16;
+
+// RK: 0 no residual, 1 residual of x's type, 2 fp32 residual
+template <typename T, int RK, int NW, int MAXC>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsArgs p) {
+  typedef typename std::conditional<RK == 2, float, T>::type R;
+  constexpr int SLOTS = NW == 1 ? 4 : 1;
+  __shared__ float part[2][NW];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int slot = NW == 1 ? wave : 0;
+  const int c0 = NW == 1 ? lane : (int)threadIdx.x;
+  constexpr int STEP = NW * 64;
+  const int D = p.D;
+  float g[MAXC][8];
+#pragma unroll
+  for (int j = 0; j < MAXC; ++j) {
+    const int k = (c0 + j * STEP) * 8;
+    csam_load8_tail(p.gamma + k, D - k, g[j]);
+  }
+  const float inv_d = 1.0f / (float)D;
+  for (int i = 0; i < p.rows; ++i) {
+    const long row = (long)blockIdx.x * SLOTS * p.rows + (long)i * SLOTS + slot;
+    if (row >= p.M) break;                                 // uniform over the waves that share the row
+    float v[MAXC][8];
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < MAXC; ++j) {
+      const int k = (c0 + j * STEP) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+      if (k < D) {
+        const bool full = p.vec && k + 8 <= D;
+        const T* xp = (const T*)p.x + row * p.ldx + k;
+        if (full) csam_load8(xp, v[j]);
+        else csam_load8_tail(xp, D - k, v[j]);
+        if constexpr (RK != 0) {
+          float r[8];
+          const R* rp = (const R*)p.r + row * p.ldr + k;
+          if (full) csam_load8(rp, r);
+          else csam_load8_tail(rp, D - k, r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] += r[e];
+          R* hp = (R*)p.h + row * p.ldh + k;
+          if (full) csam_store8(hp, v[j]);
+          else csam_store8_tail(hp, D - k, v[j]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(v[j][e], v[j][e], s);
+      }
+    }
+    s = csam_wave_sum(s);
+    if constexpr (NW > 1) {
+      if (lane == 0) part[i & 1][wave] = s;                // two buffers: a row's partials are read after the barrier that its
+      __syncthreads();                                     // writes precede, and overwritten after the next row's barrier
+      s = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) s += part[i & 1][w];
+    }
+    const float rstd = 1.0f / sqrtf(s * inv_d + p.eps);
+#pragma unroll
+    for (int j = 0; j < MAXC; ++j) {
+      const int c = c0 + j * STEP, k = c * 8;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = v[j][e] * rstd * g[j][e];
+      if (p.y_kind >= RMS_MX) {
+        if (k < p.Dp) {                                    // whole groups of 32 lanes: Dp is a multiple of 256
+          if (p.y_kind == RMS_MX + CSAM_MX_FP8) csam_mx_store8<CSAM_MX_FP8>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
+          else csam_mx_store8<CSAM_MX_FP4>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
+        }
+      } else if (k < D) {
+        const bool full = p.vec && k + 8 <= D;
+        if (p.y_kind == CSAM_DT_F16) {
+          half_t* yp = (half_t*)p.y + row * p.ldy + k;
+          if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
+        } else if (p.y_kind == CSAM_DT_BF16) {
+          bf16_t* yp = (bf16_t*)p.y + row * p.ldy + k;
+          if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
+        } else {
+          float* yp = (float*)p.y + row * p.ldy + k;
+          if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int RK>
+int rms_launch(hipStream_t st, RmsArgs& p) {
+  const int chunks = csam_cdiv(p.Dp ? p.Dp : p.D, 8);
+#define RMS_GO(NW, MAXC)                                                                              \
+  do {                                                                                                \
+    const int slots = NW == 1 ? 4 : 1;                                                                \
+    p.rows = 1;                                                                                       \
+    rms_norm_kernel<T, RK, NW, MAXC><<<csam_cdiv(p.M, (long)slots * p.rows), NW == 1 ? 256 : NW * 64, 0, st>>>(p); \
+  } while (0)
+  if (chunks <= 64) RMS_GO(1, 1);
+  else if (chunks <= 128) RMS_GO(1, 2);
+  else if (chunks <= 256) RMS_GO(1, 4);
+  else if (chunks <= 1024) RMS_GO(4, 4);
+  else RMS_GO(16, 4);
+#undef RMS_GO
+  CSAM_LAUNCH_CHECK("csam_rms_norm");
+  return CSAM_OK;
+}
+
+bool aligned(const void* p, long ld_bytes, int a) { return ((uintptr_t)p % a) == 0 && ld_bytes % a == 0; }
+int dt_bytes(int dt) { return dt == CSAM_DT_F32 ? 4 : 2; }
+bool dt_ok(int dt) { return dt == CSAM_DT_F16 || dt == CSAM_DT_F32 || dt == CSAM_DT_BF16; }
+
+// checks shared by everything that reads or writes an MX operand
+int mx_check(const char* who, const void* codes, long ldc, const void* scales, long sstride, int fmt, int M, int K) {
+  CSAM_REQUIRE(codes && scales, "%s: null operand", who);
+  CSAM_REQUIRE(fmt == CSAM_MX_FP4 || fmt == CSAM_MX_FP8, "%s: format %d is neither CSAM_MX_FP4 nor CSAM_MX_FP8", who, fmt);
+  const long Kp = (K + 255L) / 256 * 256;
+  CSAM_REQUIRE(ldc >= (fmt == CSAM_MX_FP4 ? Kp / 2 : Kp), "%s: code rows of %ld bytes are shorter than %ld padded columns", who, ldc, Kp);
+  CSAM_REQUIRE(aligned(codes, ldc, 16), "%s: codes and their row pitch have to be multiples of 16 bytes", who);
+  CSAM_REQUIRE(aligned(scales, sstride, 4) && sstride >= 4L * M, "%s: scale groups have to lie 4-byte aligned, at least 4 * rows bytes apart", who);
+  return CSAM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* codes, long ldcodes, void* scales, long scale_stride,
+                     int fmt, int M, int K) {
+  if (M == 0) return CSAM_OK;
+  CSAM_REQUIRE(x, "csam_mx_quantize: null operand");
+  CSAM_REQUIRE(M > 0 && K > 0 && ldx >= K, "csam_mx_quantize: bad sizes M %d K %d ldx %ld", M, K, ldx);
+  CSAM_REQUIRE(dt_ok(x_dtype), "csam_mx_quantize: bad dtype %d", x_dtype);
+  if (int rc = mx_check("csam_mx_quantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
+  const int nseg = csam_cdiv(K, Q_COLS);
+  const long grid = (long)nseg * csam_cdiv(M, Q_ROWS);
+  CSAM_REQUIRE(grid < (1L << 31), "csam_mx_quantize: too many elements");
+  const int vec = aligned(x, ldx * dt_bytes(x_dtype), 16);
+  hipStream_t st = (hipStream_t)stream;
+#define GO(T, F) mx_quantize_kernel<T, F><<<(unsigned)grid, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, \
+                                                                         scale_stride, M, K, nseg, vec)
+  if (fmt == CSAM_MX_FP4) {
+    if (x_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP4);
+    else if (x_dtype == CSAM_DT_F32) GO(float, CSAM_MX_FP4);
+    else GO(bf16_t, CSAM_MX_FP4);
+  } else {
+    if (x_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP8);
+    else if (x_dtype == CSAM_DT_F32) GO(float, CSAM_MX_FP8);
+    else GO(bf16_t, CSAM_MX_FP8);
+  }
+#undef GO
+  CSAM_LAUNCH_CHECK("csam_mx_quantize");
+  return CSAM_OK;
+}
+
+int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void* scales, long scale_stride, int fmt, void* y, long ldy,
+                       int y_dtype, int M, int K) {
+  if (M == 0) return CSAM_OK;
+  CSAM_REQUIRE(y, "csam_mx_dequantize: null operand");
+  CSAM_REQUIRE(M > 0 && K > 0 && ldy >= K, "csam_mx_dequantize: bad sizes M %d K %d ldy %ld", M, K, ldy);
+  CSAM_REQUIRE(dt_ok(y_dtype), "csam_mx_dequantize: bad dtype %d", y_dtype);
+  if (int rc = mx_check("csam_mx_dequantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
+  const int nseg = csam_cdiv(K, Q_COLS);
+  const long grid = (long)nseg * csam_cdiv(M, Q_ROWS);
+  CSAM_REQUIRE(grid < (1L << 31), "csam_mx_dequantize: too many elements");
+  const int vec = aligned(y, ldy * dt_bytes(y_dtype), 16);
+  hipStream_t st = (hipStream_t)stream;
+#define GO(T, F) mx_dequantize_kernel<T, F><<<(unsigned)grid, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, \
+                                                                           scale_stride, (T*)y, ldy, M, K, nseg, vec)
+  if (fmt == CSAM_MX_FP4) {
+    if (y_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP4);
+    else if (y_dtype == CSAM_DT_F32) GO(float, CSAM_MX_FP4);
+    else GO(bf16_t, CSAM_MX_FP4);
+  } else {
+    if (y_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP8);
+    else if (y_dtype == CSAM_DT_F32) GO(float, CSAM_MX_FP8);
+    else GO(bf16_t, CSAM_MX_FP8);
+  }
+#undef GO
+  CSAM_LAUNCH_CHECK("csam_mx_dequantize");
+  return CSAM_OK;
+}
+
+static int rms_any(hipStream_t st, RmsArgs& p, int x_dtype, int r_dtype, const char* who) {
+  CSAM_REQUIRE(p.x && p.gamma && p.y, "%s: null operand", who);
+  CSAM_REQUIRE((p.r == nullptr) == (p.h == nullptr), "%s: the residual and the sum's output come together", who);
+  CSAM_REQUIRE(p.M > 0 && p.D > 0 && p.D <= 32768, "%s: bad sizes M %d D %d (D <= 32768)", who, p.M, p.D);
+  CSAM_REQUIRE(p.ldx >= p.D && (!p.r || (p.ldr >= p.D && p.ldh >= p.D)), "%s: a row pitch is shorter than the row", who);
+  CSAM_REQUIRE(dt_ok(x_dtype), "%s: bad dtype %d", who, x_dtype);
+  CSAM_REQUIRE(!p.r || r_dtype == x_dtype || r_dtype == CSAM_DT_F32, "%s: the residual is fp32 or of x's type", who);
+  CSAM_REQUIRE(p.eps > 0.f, "%s: eps has to be positive", who);
+  p.vec = aligned(p.x, p.ldx * dt_bytes(x_dtype), 16) &&
+          (!p.r || (aligned(p.r, p.ldr * dt_bytes(r_dtype), 16) && aligned(p.h, p.ldh * dt_bytes(r_dtype), 16)));
+  if (p.y_kind < RMS_MX) p.vec = p.vec && aligned(p.y, p.ldy * dt_bytes(p.y_kind), 16);
+  const int rk = !p.r ? 0 : (r_dtype == CSAM_DT_F32 && x_dtype != CSAM_DT_F32) ? 2 : 1;
+#define GO(T) return rk == 0 ? rms_launch<T, 0>(st, p) : rk == 1 ? rms_launch<T, 1>(st, p) : rms_launch<T, 2>(st, p)
+  if (x_dtype == CSAM_DT_F16) GO(half_t);
+  if (x_dtype == CSAM_DT_BF16) GO(bf16_t);
+#undef GO
+  return rk == 0 ? rms_launch<float, 0>(st, p) : rms_launch<float, 1>(st, p);
+}
+
+int csam_rms_norm(void* stream, const void* x, long ldx, int x_dtype, const void* residual, long ldr, int r_dtype, void* h, long ldh,
+                  const float* gamma, float eps, void* y, long ldy, int y_dtype, int M, int D) {
+  if (M == 0) return CSAM_OK;
+  CSAM_REQUIRE(dt_ok(y_dtype) && ldy >= D, "csam_rms_norm: bad output dtype %d or row pitch %ld", y_dtype, ldy);
+  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0, 0, 1};
+  return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm");
+}
+
+int csam_rms_norm_mx(void* stream, const void* x, long ldx, int x_dtype, const void* residual, long ldr, int r_dtype, void* h, long ldh,
+                     const float* gamma, float eps, void* codes, long ldcodes, void* scales, long scale_stride, int fmt, int M, int D) {
+  if (M == 0) return CSAM_OK;
+  CSAM_REQUIRE(D > 0, "csam_rms_norm_mx: bad width %d", D);
+  if (int rc = mx_check("csam_rms_norm_mx", codes, ldcodes, scales, scale_stride, fmt, M, D)) return rc;
+  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, codes, ldcodes, RMS_MX + fmt, (uint8_t*)scales, scale_stride, M, D,
+               csam_cdiv(D, 256) * 256, 0, 1};
+  return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm_mx");
+}
+
+}  // extern "C"

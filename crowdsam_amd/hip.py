@@ -8,6 +8,7 @@ imported from here).
 """
 import ctypes
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -99,6 +100,12 @@ SIGNATURES = {
     "csam_resize_linear_u8": [_P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _P],
     "csam_u8hwc_to_f32chw": [_P, _P, _I, _I, _P],
     "csam_pil_resample_u8": [_P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P],
+    "csam_mx_quantize": [_P, _P, _L, _I, _P, _L, _P, _L, _I, _I, _I],
+    "csam_mx_dequantize": [_P, _P, _L, _P, _L, _I, _P, _L, _I, _I, _I],
+    "csam_mx_gemm": [_P, _P, _L, _P, _L, _I, _P, _L, _P, _L, _P, _L, _I, _P, _P, _L, _I, _I, _I, _I, _I],
+    "csam_rms_norm": [_P, _P, _L, _I, _P, _L, _I, _P, _L, _P, _F, _P, _L, _I, _I, _I],
+    "csam_rms_norm_mx": [_P, _P, _L, _I, _P, _L, _I, _P, _L, _P, _F, _P, _L, _P, _L, _I, _I, _I],
+    "csam_rotary": [_P, _P, _L, _I, _P, _L, _I, _I, _P, _L, _I, _P, _L, _I, _I, _I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _I, _I],
 }
 LONG_RETURNS = {
     "csam_coco_rle_string": [_P, _L, _P, _L],
@@ -1165,3 +1172,243 @@ def coco_rle_string(counts):
     if n < 0:
         raise RuntimeError("csam_coco_rle_string: buffer too small")
     return buf.raw[:n].decode("ascii")
+
+
+# ----------------------------------------------------------------------------------------------
+# microscaled (MX) operands, RMS norm, rotary positions.  These take fp16, bfloat16 and fp32 tensors on any HIP device, work on the
+# current stream of that device, allocate nothing but their outputs, and raise ValueError for arguments they do not take.
+# ----------------------------------------------------------------------------------------------
+_DT3 = {torch.float16: DT_F16, torch.float32: DT_F32, torch.bfloat16: 2}
+_MX = {"fp4": 0, "fp8": 1}
+
+
+class MxTensor(NamedTuple):
+    """A microscaled operand of ``rows`` x ``K`` values: ``codes`` uint8 [rows, Kp / 2] (``fmt`` "fp4": E2M1, element 2i in the low
+    nibble of byte i) or [rows, Kp] ("fp8": E4M3), ``scales`` uint8 [Kp / 128, rows, 4]: the E8M0 byte of block b (columns 32b ..
+    32b + 31) of row r at [b // 4, r, b % 4].  Kp is K rounded up to a multiple of 256; codes behind K are zero.  Rows may be sliced:
+    ``q.rows(i, j)``."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    fmt: str
+    K: int
+
+    def rows(self, i, j):
+        return MxTensor(self.codes[i:j], self.scales[:, i:j], self.fmt, self.K)
+
+
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _mx_padded(K):
+    return -(-K // 256) * 256
+
+
+def _mx_empty(rows, K, fmt, device):
+    Kp = _mx_padded(K)
+    return MxTensor(torch.empty((rows, Kp // 2 if fmt == "fp4" else Kp), dtype=torch.uint8, device=device),
+                    torch.empty((Kp // 128, rows, 4), dtype=torch.uint8, device=device), fmt, K)
+
+
+def _mx_check(q, who, name):
+    """(code row pitch, scale group pitch) of an operand whose shapes, dtypes and strides are what the kernels read."""
+    c, s = q.codes, q.scales
+    _need(q.fmt in _MX, f"{who}: {name} has format {q.fmt!r}, not 'fp4' or 'fp8'")
+    _need(q.K > 0, f"{who}: {name} has K = {q.K}")
+    Kp = _mx_padded(q.K)
+    _need(c.dtype == torch.uint8 and s.dtype == torch.uint8, f"{who}: {name} has {c.dtype} codes and {s.dtype} scales, not uint8")
+    _need(c.dim() == 2 and c.shape[1] == (Kp // 2 if q.fmt == "fp4" else Kp),
+          f"{who}: {name} has codes of shape {tuple(c.shape)}, not [rows, {Kp // 2 if q.fmt == 'fp4' else Kp}] (K = {q.K} padded to {Kp})")
+    rows = c.shape[0]
+    _need(tuple(s.shape) == (Kp // 128, rows, 4), f"{who}: {name} has scales of shape {tuple(s.shape)}, not {(Kp // 128, rows, 4)}")
+    ldc = c.stride(0) if rows > 1 else c.shape[1]
+    ss = s.stride(0) if Kp > 128 else 4 * rows
+    _need(rows == 0 or (c.stride(1) == 1 and ldc >= c.shape[1] and ldc % 16 == 0 and c.data_ptr() % 16 == 0),
+          f"{who}: {name} has code rows that are not contiguous, or not 16-byte aligned")
+    _need(rows == 0 or (s.stride(2) == 1 and (rows == 1 or s.stride(1) == 4) and ss >= 4 * rows and ss % 4 == 0 and s.data_ptr() % 4 == 0),
+          f"{who}: {name} has scales whose rows of a group are not 4 bytes apart")
+    return ldc, ss
+
+
+def _mat(t, who, name, cols=None, rows=None):
+    """Row pitch in elements of a [rows, cols] matrix with contiguous rows."""
+    _need(t.dim() == 2, f"{who}: {name} has {t.dim()} dimensions, not 2")
+    _need(t.dtype in _DT3, f"{who}: {name} is {t.dtype}, not float16, bfloat16 or float32")
+    _need(max(t.shape) < 1 << 31, f"{who}: {name} has {max(t.shape)} rows or columns")
+    _need((rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols),
+          f"{who}: {name} has shape {tuple(t.shape)}, not {(t.shape[0] if rows is None else rows, t.shape[1] if cols is None else cols)}")
+    _need(t.numel() == 0 or t.shape[1] == 1 or t.stride(1) == 1, f"{who}: rows of {name} are not contiguous")
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    _need(t.numel() == 0 or ld >= t.shape[1], f"{who}: rows of {name} overlap")
+    return ld
+
+
+def _vec_f32(t, who, name, n):
+    _need(t.dtype == torch.float32 and tuple(t.shape) == (n,) and t.is_contiguous(), f"{who}: {name} has to be a contiguous float32 [{n}]")
+
+
+def _call_on(who, tensors, name, *args):
+    """Calls an entry on the current stream of the device that all of the tensors are on."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise ValueError(f"{who}: tensors are on {dev}; there is no CPU form")
+    if dev.index == torch.cuda.current_device():
+        call(name, _stream(), *args)
+    else:
+        with torch.cuda.device(dev):
+            call(name, _stream(), *args)
+
+
+def mx_quantize(x, fmt="fp4"):
+    """``x`` [M, K] (fp16, bfloat16 or fp32, contiguous rows) as an ``MxTensor``: per block of 32 columns the scale
+    2^(floor(log2 amax) - emax), emax 2 ("fp4") or 8 ("fp8"), and every value over its scale rounded to nearest even, saturated at 6 or
+    448.  A block with a NaN or an infinity reads back as NaN."""
+    _need(fmt in _MX, f"mx_quantize: format {fmt!r} is not 'fp4' or 'fp8'")
+    ld = _mat(x, "mx_quantize", "x")
+    M, K = x.shape
+    _need(K > 0, "mx_quantize: x has no columns")
+    q = _mx_empty(M, K, fmt, x.device)
+    _call_on("mx_quantize", (x,), "csam_mx_quantize", _ptr(x), ld, _DT3[x.dtype], _ptr(q.codes), q.codes.shape[1], _ptr(q.scales), 4 * M,
+             _MX[fmt], M, K)
+    return q
+
+
+def mx_dequantize(q, out_dtype=torch.float32):
+    """The values [rows, K] an ``MxTensor`` stands for, rounded to ``out_dtype`` (exact in fp32; in bfloat16 too but for values below its
+    smallest)."""
+    _need(out_dtype in _DT3, f"mx_dequantize: no output in {out_dtype}")
+    ldc, ss = _mx_check(q, "mx_dequantize", "q")
+    M = q.codes.shape[0]
+    y = torch.empty((M, q.K), dtype=out_dtype, device=q.codes.device)
+    _call_on("mx_dequantize", (q.codes, q.scales), "csam_mx_dequantize", _ptr(q.codes), ldc, _ptr(q.scales), ss, _MX[q.fmt], _ptr(y), q.K,
+             _DT3[out_dtype], M, q.K)
+    return y
+
+
+def mx_gemm(a, w, out=None, bias=None, act=ACT_NONE, residual=None, out_dtype=torch.float16):
+    """out[M, N] = act(a w^T + bias) + residual of two ``MxTensor``s: ``a`` [M, K] in "fp4" or "fp8", ``w`` [N, K] in "fp4"; fp32 sums,
+    rounded once.  ``bias`` fp32 [N]; ``residual`` [M, N] fp16 / bfloat16 / fp32; ``out`` may be the residual.  The kernel and with it the
+    order of the sum depend on the sizes: rows are not bitwise independent of M."""
+    who = "mx_gemm"
+    _need(w.fmt == "fp4", f"{who}: w is in {w.fmt!r}; only 'fp4' weights are multiplied")
+    _need(a.K == w.K, f"{who}: a has K = {a.K}, w has K = {w.K}")
+    _need(a.K <= 1 << 20, f"{who}: K = {a.K} is over 2^20")
+    _need(act in (ACT_NONE, ACT_GELU, ACT_RELU), f"{who}: activation {act!r}")
+    lda, ass = _mx_check(a, who, "a")
+    ldw, wss = _mx_check(w, who, "w")
+    M, N = a.codes.shape[0], w.codes.shape[0]
+    ldr, r_dt = 0, 0
+    if residual is not None:
+        ldr, r_dt = _mat(residual, who, "residual", N, M), _DT3[residual.dtype]
+    if bias is not None:
+        _vec_f32(bias, who, "bias", N)
+    if out is None:
+        _need(out_dtype in _DT3, f"{who}: no output in {out_dtype}")
+        out = torch.empty((M, N), dtype=out_dtype, device=a.codes.device)
+        ldo = N
+    else:
+        ldo = _mat(out, who, "out", N, M)
+    _call_on(who, (a.codes, a.scales, w.codes, w.scales, out, bias, residual), "csam_mx_gemm", _ptr(a.codes), lda, _ptr(a.scales), ass,
+             _MX[a.fmt], _ptr(w.codes), ldw, _ptr(w.scales), wss, _ptr(out), ldo, _DT3[out.dtype], _ptr(bias), _ptr(residual), ldr, r_dt,
+             act, M, N, a.K)
+    return out
+
+
+def rms_norm(x, gamma, eps, residual=None, h_out=None, out_dtype=torch.float16):
+    """y = h * rsqrt(mean(h^2) + eps) * gamma over the rows of h = x + residual; ``x`` [M, D] fp16 / bfloat16 / fp32, ``gamma`` fp32 [D],
+    D <= 32768.  ``out_dtype``: a float type, or "fp8" / "fp4" for an ``MxTensor``.  Without a residual returns y; with one (fp32, or x's
+    type) returns (y, h), h in the residual's type and in ``h_out`` if given, which may be the residual itself."""
+    who = "rms_norm"
+    ldx = _mat(x, who, "x")
+    M, D = x.shape
+    _need(0 < D <= 32768, f"{who}: rows of {D} values (1 .. 32768)")
+    _need(eps > 0, f"{who}: eps has to be positive, got {eps}")
+    _vec_f32(gamma, who, "gamma", D)
+    _need(residual is not None or h_out is None, f"{who}: h_out without a residual")
+    ldr = ldh = r_dt = 0
+    if residual is not None:
+        _need(residual.dtype in (x.dtype, torch.float32), f"{who}: the residual is {residual.dtype}; it has to be {x.dtype} or float32")
+        ldr, r_dt = _mat(residual, who, "residual", D, M), _DT3[residual.dtype]
+        if h_out is None:
+            h_out = torch.empty((M, D), dtype=residual.dtype, device=x.device)
+        _need(h_out.dtype == residual.dtype, f"{who}: h_out is {h_out.dtype}, the residual {residual.dtype}")
+        ldh = _mat(h_out, who, "h_out", D, M)
+    head = (_ptr(x), ldx, _DT3[x.dtype], _ptr(residual), ldr, r_dt, _ptr(h_out), ldh, _ptr(gamma), float(eps))
+    if out_dtype in _MX:
+        y = _mx_empty(M, D, out_dtype, x.device)
+        _call_on(who, (x, gamma, residual, h_out), "csam_rms_norm_mx", *head, _ptr(y.codes), y.codes.shape[1], _ptr(y.scales), 4 * M,
+                 _MX[out_dtype], M, D)
+    else:
+        _need(out_dtype in _DT3, f"{who}: no output in {out_dtype}")
+        y = torch.empty((M, D), dtype=out_dtype, device=x.device)
+        _call_on(who, (x, gamma, residual, h_out), "csam_rms_norm", *head, _ptr(y), D, _DT3[out_dtype], M, D)
+    return y if residual is None else (y, h_out)
+
+
+def rotary_frequencies(sections, theta=10000.0, device="cuda"):
+    """(freq fp64 [pairs], axis int32 [pairs]) of ``rotary`` for ``sections[i]`` pairs of axis i, each axis with the geometric spectrum
+    theta^(-j / sections[i])."""
+    _need(len(sections) > 0 and all(n > 0 for n in sections), f"rotary_frequencies: sections {sections}")
+    freq = [float(theta) ** (-j / n) for n in sections for j in range(n)]
+    axis = [i for i, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(freq, dtype=torch.float64, device=device), torch.tensor(axis, dtype=torch.int32, device=device)
+
+
+def _heads(t, who, name, T, hd, written=False):
+    _need(t.dim() == 3 and t.shape[0] == T and t.shape[2] == hd and t.shape[1] > 0,
+          f"{who}: {name} has shape {tuple(t.shape)}, not [{T}, heads, {hd}]")
+    hs = t.stride(1) if t.shape[1] > 1 else hd
+    _need(T == 0 or ((hd == 1 or t.stride(2) == 1) and hd <= hs < 1 << 31), f"{who}: elements of a head of {name} are not contiguous, or heads overlap")
+    ld, H = (t.stride(0) if T > 1 else 0), t.shape[1]
+    _need(not written or T <= 1 or ld >= (H - 1) * hs + hd or (ld >= hd and hs >= (T - 1) * ld + hd), f"{who}: tokens of {name} overlap")
+    return ld, hs
+
+
+def rotary(q, k, pos, freq, axis, interleaved=False, q_out=None, k_out=None):
+    """Rotary positions with several axes: pair p of every head of token t turns by ``pos[axis[p], t] * freq[p]`` radians.  ``q`` [T, Hq, hd]
+    and ``k`` [T, Hk, hd] (or None) fp16 / bfloat16 / fp32 with contiguous heads, any row and head pitch -- e.g. views of a qkv matrix;
+    ``pos`` int32 or fp32 [axes, Tp], T a multiple of Tp (images of a batch that share a grid); ``freq`` fp64 and ``axis`` int32 [pairs]
+    (``rotary_frequencies``).  Pairs are elements (p, p + pairs) of a head, or (2p, 2p + 1) if ``interleaved``; elements behind the pairs are
+    copied.  Returns (q_out, k_out), new tensors unless given; an output may be its input.  The gradient with respect to q and k is this
+    call on the output's gradient with ``-pos``."""
+    who = "rotary"
+    _need(q.dim() == 3, f"{who}: q has {q.dim()} dimensions, not 3")
+    T, Hq, hd = q.shape
+    _need(T < 1 << 31 and hd > 0, f"{who}: q has shape {tuple(q.shape)}")
+    _need(q.dtype in _DT3, f"{who}: q is {q.dtype}, not float16, bfloat16 or float32")
+    P = freq.numel()
+    _need(freq.dtype == torch.float64 and axis.dtype == torch.int32 and tuple(freq.shape) == tuple(axis.shape) == (P,)
+          and freq.is_contiguous() and axis.is_contiguous(), f"{who}: freq has to be float64 [pairs], axis int32 [pairs], both contiguous")
+    _need(0 < P and 2 * P <= hd, f"{who}: {P} pairs do not fit heads of {hd}")
+    _need(pos.dim() == 2 and pos.dtype in (torch.int32, torch.float32) and pos.shape[0] > 0, f"{who}: pos has to be int32 or float32 [axes, tokens]")
+    A, Tp = pos.shape
+    _need(T == 0 or (Tp > 0 and T % Tp == 0), f"{who}: {T} tokens are not a multiple of {Tp} positions")
+    _need(T == 0 or ((Tp == 1 or pos.stride(1) == 1) and (A == 1 or pos.stride(0) >= Tp)), f"{who}: positions of an axis are not contiguous")
+    if q_out is None:
+        q_out = torch.empty((T, Hq, hd), dtype=q.dtype, device=q.device)
+    outs = [(q, q_out, "q")]
+    if k is not None:
+        _heads(k, who, "k", T, hd)
+        if k_out is None:
+            k_out = torch.empty((T, k.shape[1], hd), dtype=k.dtype, device=k.device)
+        outs.append((k, k_out, "k"))
+    else:
+        _need(k_out is None, f"{who}: k_out without k")
+    geo = []
+    for src, dst, name in outs:
+        _need(src.dtype == q.dtype and dst.dtype == q.dtype, f"{who}: {name} is {src.dtype} and {name}_out {dst.dtype}, q is {q.dtype}")
+        _need(src.shape == dst.shape, f"{who}: {name}_out has shape {tuple(dst.shape)}, not {tuple(src.shape)}")
+        geo.append((_heads(src, who, name, T, hd), _heads(dst, who, name + "_out", T, hd, True), src.shape[1]))
+    (q_ld, q_hs), (qo_ld, qo_hs), _ = geo[0]
+    if k is not None:
+        (k_ld, k_hs), (ko_ld, ko_hs), Hk = geo[1]
+    else:
+        k_ld = k_hs = ko_ld = ko_hs = Hk = 0
+    _call_on(who, (q, k, q_out, k_out, pos, freq, axis), "csam_rotary", _ptr(q), q_ld, q_hs, _ptr(q_out), qo_ld, qo_hs, Hq, _ptr(k), k_ld,
+             k_hs, _ptr(k_out), ko_ld, ko_hs, Hk, _DT3[q.dtype], _ptr(pos), max(pos.stride(0) if A > 1 else Tp, 1),
+             int(pos.dtype == torch.float32), _ptr(freq), _ptr(axis), A, P, int(bool(interleaved)), T, Tp, hd)
+    return q_out, k_out

@@ -34,6 +34,8 @@
  *               kernels' tests compare against it -- or from a test directly: csam_attn_t2i, csam_attn_i2t,
  *               csam_attn_t2i_workspace_bytes, csam_hyper_masks, csam_ln64_gelu, csam_softmax_stats, csam_pool_adjoint,
  *               csam_post_finalize, csam_i2t_rank_workspace_bytes.
+ *   OPERATOR    called by programs of their own beside the detector, not by it: csam_mx_quantize, csam_mx_dequantize, csam_mx_gemm,
+ *               csam_rms_norm, csam_rms_norm_mx, csam_rotary.
  * Entries that neither a product path nor a test called were dropped in round 6: csam_rle_count, csam_rle_write,
  * csam_rle_count_idx, csam_rle_write_idx (the *_box forms with boxes == NULL are they), csam_pool_adjoint_v2.
  */
@@ -100,6 +102,47 @@ int csam_linear_f32(void* stream, const float* A, long lda, const float* W, long
 int csam_linear_f32_batched(void* stream, const float* A, long lda, long strideA, const float* W, long ldw,
                             long strideW, const float* bias, long strideBias, float* C, long ldc, long strideC,
                             int M, int N, int K, int act, int batch);
+
+/* ---- microscaled (MX) operands: quantisation, product, and the norm that feeds it.  Entries of their own beside the fp16
+ * projections (the reference computes every nn.Linear in fp32: image_encoder.py:227,238; common.py:25-26); no default path of the
+ * detector calls them.
+ * An MX operand of R rows and K columns, Kp = K rounded up to a multiple of 256:
+ *   codes   CSAM_MX_FP4 (E2M1): [R][ldcodes] bytes, Kp / 2 used, element 2i in the low nibble of byte i;
+ *           CSAM_MX_FP8 (E4M3): [R][ldcodes] bytes, Kp used.  Columns K .. Kp-1 hold zero codes.
+ *           16-byte aligned, ldcodes a multiple of 16;
+ *   scales  E8M0 bytes, 2^(s - 127), 255 = NaN: block b = columns 32b .. 32b+31 of row r at scales[(b / 4) * scale_stride + r * 4 + b % 4];
+ *           4-byte aligned, scale_stride a multiple of 4 and >= 4 * R.
+ * f16 / f32 / bf16 = CSAM_DT_F16 / _F32 / _BF16 in these entries and csam_rotary only. */
+#define CSAM_DT_BF16 2
+#define CSAM_MX_FP4 0
+#define CSAM_MX_FP8 1
+/* s = max(floor(log2 amax) - emax, -127) + 127 with emax 2 (E2M1) / 8 (E4M3), codes = x / 2^(s-127) rounded to nearest even and
+ * saturated at 6 / 448.  A block that holds a NaN or an infinity gets s = 255 (and zero codes): all of it reads as NaN.  A block whose
+ * amax is zero or subnormal gets s = 0. */
+int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* codes, long ldcodes, void* scales, long scale_stride,
+                     int fmt, int M, int K);
+int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void* scales, long scale_stride, int fmt, void* y, long ldy,
+                       int y_dtype, int M, int K);
+/* C[M,N] = act(A W^T + bias[n]) + residual[m,n]; A in either format, W in CSAM_MX_FP4, fp32 sums, one rounding to c_dtype.  bias
+ * (fp32 [N]) and residual (f16 / f32 / bf16) may be NULL; C may be the residual itself.  K is the unpadded width; any M, N. */
+int csam_mx_gemm(void* stream, const void* A, long lda, const void* A_scales, long a_scale_stride, int a_fmt, const void* W, long ldw,
+                 const void* W_scales, long w_scale_stride, void* C, long ldc, int c_dtype, const float* bias, const void* residual,
+                 long ldr, int r_dtype, int act, int M, int N, int K);
+/* h = x + residual (fp32), y = h * rsqrt(mean(h^2) + eps) * gamma: h is written in the residual's type (fp32, or x's), y is computed from
+ * the unrounded sum.  residual and h both NULL: y only; h may be the residual itself.  D <= 32768, eps > 0.  The _mx form writes y as
+ * an MX operand (columns behind D are zero). */
+int csam_rms_norm(void* stream, const void* x, long ldx, int x_dtype, const void* residual, long ldr, int r_dtype, void* h, long ldh,
+                  const float* gamma, float eps, void* y, long ldy, int y_dtype, int M, int D);
+int csam_rms_norm_mx(void* stream, const void* x, long ldx, int x_dtype, const void* residual, long ldr, int r_dtype, void* h, long ldh,
+                     const float* gamma, float eps, void* codes, long ldcodes, void* scales, long scale_stride, int fmt, int M, int D);
+/* Rotary positions with several axes on the heads of q and (Hk > 0) k: pair p of a head turns by pos[axis[p]][t % T_pos] * freq[p]
+ * radians, (a, b) -> (a cos - b sin, a sin + b cos).  Pairs are elements (p, p + pairs), or (2p, 2p + 1) if interleaved; elements from
+ * 2 * pairs on are copied.  q [T][Hq][head_dim] with row pitch ldq and head pitch hsq in elements (k alike); the outputs may be the
+ * inputs.  pos int32 or fp32 [axes][pos_stride], T a multiple of T_pos; freq fp64 [pairs]; axis int32 [pairs], clamped to 0 .. axes-1.
+ * Angles are formed and reduced in fp64.  The adjoint is the call with negated positions. */
+int csam_rotary(void* stream, const void* q, long ldq, int hsq, void* q_out, long ldqo, int hsqo, int Hq, const void* k, long ldk, int hsk,
+                void* k_out, long ldko, int hsko, int Hk, int dtype, const void* pos, long pos_stride, int pos_is_f32, const double* freq,
+                const int* axis, int axes, int pairs, int interleaved, int T, int T_pos, int head_dim);
 
 /* ---- encoder-side streaming kernels */
 /* nn.LayerNorm / LayerNorm2d on token-major rows (image_encoder.py:168,180; common.py:38-43;

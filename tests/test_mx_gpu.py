@@ -1,0 +1,244 @@
+"""Microscaled quantisation and product against their definition in float64."""
+import pytest
+import torch
+
+import mx_ref
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24                      # half an fp32 step
+DTS = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def same(q, codes, scales):
+    assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), scales)
+
+
+def equal(a, b):
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def awkward(m, k, dtype, seed):
+    """Rows whose blocks span the type's range, with ties, signed zeros, zero blocks and subnormals."""
+    g = gen(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-12, 12, (m, -(-k // 32)), generator=g).float()).repeat_interleave(32, 1)[:, :k]
+    flat = x.view(-1)
+    ties = torch.tensor([0.25, -0.75, 1.25, 1.75, 2.5, -3.5, 5.0, 6.0, 7.0, 17.0, 19.0, 464.0, 0.0, -0.0])
+    n = min(flat.numel(), 500)
+    flat[torch.randperm(flat.numel(), generator=g)[:n]] = ties[torch.randint(0, len(ties), (n,), generator=g)]
+    x[m // 2, :] = 0.0
+    if dtype == torch.float32:
+        x[0, : min(k, 64)] *= 2.0 ** -140
+        x[-1, : min(k, 32)] = torch.linspace(-3.4e38, 3.4e38, min(k, 32))
+    if dtype == torch.bfloat16:
+        x[0, : min(k, 64)] *= 2.0 ** -130
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 32), (3, 33), (33, 250), (31, 256), (65, 1001), (130, 1280)])
+def test_quantize_is_the_definition(cuda, fmt, dtype, m, k):
+    from crowdsam_amd import hip
+    x = awkward(m, k, dtype, m * k)
+    q = hip.mx_quantize(x.to(cuda), fmt)
+    assert q.K == k and q.fmt == fmt
+    same(q, *mx_ref.quantize(x, fmt))
+    v = mx_ref.values(q)
+    assert equal(hip.mx_dequantize(q).cpu().double(), v)
+    for dt in (torch.float16, torch.bfloat16):
+        assert equal(hip.mx_dequantize(q, out_dtype=dt).cpu(), v.float().to(dt))
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8"])
+def test_quantize_strided_rows_and_nan_blocks(cuda, fmt):
+    from crowdsam_amd import hip
+    base = torch.randn(40, 700, generator=gen(5)).half()
+    base[3, 40] = float("nan")
+    base[7, 64] = float("inf")
+    base[9, 95] = float("-inf")
+    for cut in (slice(0, 640), slice(1, 641), slice(8, 328), slice(3, 100)):       # aligned and unaligned rows
+        x = base[:, cut]
+        q = hip.mx_quantize(base.to(cuda)[:, cut], fmt)
+        same(q, *mx_ref.quantize(x, fmt))
+        v = hip.mx_dequantize(q).cpu()
+        blocks = torch.isfinite(torch.nn.functional.pad(x.float(), (0, -x.shape[1] % 32))).view(40, -1, 32).all(2)
+        assert torch.equal(torch.isnan(v), ~blocks.repeat_interleave(32, 1)[:, :x.shape[1]])
+
+
+def test_empty_operands(cuda):
+    from crowdsam_amd import hip
+    q = hip.mx_quantize(torch.zeros(0, 96, device=cuda), "fp8")
+    assert q.codes.shape == (0, 256) and hip.mx_dequantize(q).shape == (0, 96)
+    w = hip.mx_quantize(torch.ones(5, 96, device=cuda), "fp4")
+    assert hip.mx_gemm(q, w).shape == (0, 5)
+    assert hip.mx_gemm(hip.mx_quantize(torch.ones(5, 96, device=cuda), "fp8"), w.rows(0, 0)).shape == (5, 0)
+    y, h = hip.rms_norm(torch.zeros(0, 64, device=cuda), torch.ones(64, device=cuda), 1e-6, residual=torch.zeros(0, 64, device=cuda))
+    assert y.shape == h.shape == (0, 64)
+
+
+def operands(m, n, k, fa, seed):
+    g = gen(seed)
+    a = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-3, 4, (m, 1), generator=g).float())
+    w = torch.randn(n, k, generator=g) * 0.05 + torch.arange(n).view(n, 1) * 1e-3
+    return a, w
+
+
+def product_ref(hip, qa, qw, bias, act, residual, out_dtype):
+    """(float64 result, bound).  n fp32 additions in any order are off by at most n U sum |a w|, taken twice: the matrix unit may cut
+    where it is not said to round.  GELU: slope at most 1.13, its erf is off by 1.5e-7 (half of it times |x|); every later operation
+    and the store round once."""
+    va, vw = mx_ref.values(qa), mx_ref.values(qw)
+    c = va @ vw.t()
+    tol = 2 * U * va.shape[1] * (va.abs() @ vw.abs().t())
+    if bias is not None:
+        c = c + bias.double()
+        tol = tol + U * c.abs()
+    if act == hip.ACT_GELU:
+        x = c
+        c = x * 0.5 * torch.special.erfc(-x / 2 ** 0.5)
+        tol = 1.13 * tol + 1.0e-7 * x.abs() + 4 * U * c.abs()
+    elif act == hip.ACT_RELU:
+        c = c.clamp(min=0)
+    if residual is not None:
+        c = c + residual.double()
+        tol = tol + U * c.abs()
+    tol = tol + torch.finfo(out_dtype).eps / 2 * c.abs() + torch.finfo(out_dtype).smallest_normal * torch.finfo(out_dtype).eps
+    return c, tol * (1 + 2.0 ** -7)           # the bound itself is taken at the exact value, not at the rounded one
+
+
+def close(out, ref, tol):
+    d = (out.cpu().double() - ref).abs()
+    assert bool((d <= tol).all()), float((d / tol).max())
+
+
+@pytest.mark.parametrize("fa", ["fp4", "fp8"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 16, 32), (1, 130, 256), (7, 33, 500), (15, 16, 512), (16, 250, 2048), (17, 64, 1000), (33, 31, 256),
+                                   (64, 128, 1280), (65, 129, 256), (127, 200, 300), (130, 128, 512), (300, 384, 1280), (513, 260, 1001),
+                                   (1000, 1024, 256)])
+def test_gemm_matches_float64(cuda, fa, m, n, k):
+    from crowdsam_amd import hip
+    a, w = operands(m, n, k, fa, m + n + k)
+    qa, qw = hip.mx_quantize(a.to(cuda), fa), hip.mx_quantize(w.to(cuda), "fp4")
+    out = hip.mx_gemm(qa, qw, out_dtype=torch.float32)
+    close(out, *product_ref(hip, qa, qw, None, 0, None, torch.float32))
+
+
+@pytest.mark.parametrize("fa", ["fp4", "fp8"])
+@pytest.mark.parametrize("m", [5, 70, 300])
+@pytest.mark.parametrize("act", [0, 1, 2])
+@pytest.mark.parametrize("out_dtype,res_dtype", [(torch.float16, None), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32),
+                                                 (torch.float16, torch.float32), (torch.float32, torch.float16)])
+def test_gemm_epilogues(cuda, fa, m, act, out_dtype, res_dtype):
+    from crowdsam_amd import hip
+    n, k = 200, 320
+    a, w = operands(m, n, k, fa, 11 + m)
+    bias = torch.randn(n, generator=gen(2))
+    res = None if res_dtype is None else torch.randn(m, n, generator=gen(3)).to(res_dtype)
+    qa, qw = hip.mx_quantize(a.to(cuda), fa), hip.mx_quantize(w.to(cuda), "fp4")
+    out = hip.mx_gemm(qa, qw, bias=bias.to(cuda), act=act, residual=None if res is None else res.to(cuda), out_dtype=out_dtype)
+    assert out.dtype == out_dtype
+    close(out, *product_ref(hip, qa, qw, bias, act, res, out_dtype))
+
+
+@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("cols", [129, 132])
+def test_gemm_strides_in_place_and_slices(cuda, m, cols):
+    """Rows of an operand, outputs and residuals that are windows of larger matrices, and the residual overwritten in place; what lies
+    around the window keeps its values."""
+    from crowdsam_amd import hip
+    k = 300
+    a, w = operands(m + 9, cols + 7, k, "fp8", 4)
+    qa, qw = hip.mx_quantize(a.to(cuda), "fp8").rows(5, 5 + m), hip.mx_quantize(w.to(cuda), "fp4").rows(7, 7 + cols)
+    for off in (4, 3):
+        big = torch.randn(m + 4, cols + 9, generator=gen(8)).to(cuda)
+        before = big.clone()
+        win = big[2:2 + m, off:off + cols]
+        hip.mx_gemm(qa, qw, out=win, residual=win)
+        close(win, *product_ref(hip, qa, qw, None, 0, before[2:2 + m, off:off + cols].cpu(), torch.float32))
+        big[2:2 + m, off:off + cols] = before[2:2 + m, off:off + cols]
+        assert torch.equal(big, before)
+
+
+@pytest.mark.parametrize("m", [4, 150])
+def test_gemm_scale_range_and_nan(cuda, m):
+    from crowdsam_amd import hip
+    n, k = 140, 256
+    a, w = operands(m, n, k, "fp4", 21)
+    a = a * torch.exp2(torch.linspace(-90, 20, m)).view(m, 1)
+    a[2, 40] = float("nan")
+    w[3, 200] = float("inf")
+    qa, qw = hip.mx_quantize(a.to(cuda), "fp4"), hip.mx_quantize(w.to(cuda), "fp4")
+    out = hip.mx_gemm(qa, qw, out_dtype=torch.float32).cpu()
+    bad = torch.zeros(m, n, dtype=torch.bool)
+    bad[2, :] = True
+    bad[:, 3] = True
+    assert torch.equal(torch.isnan(out), bad)
+    ref, tol = product_ref(hip, qa, qw, None, 0, None, torch.float32)
+    assert bool(((out.double() - ref).abs() <= tol)[~bad].all())
+
+
+def test_gemm_large_offsets(cuda):
+    """Codes and outputs whose offsets pass 32 bits: the last rows of a tall operand against the same rows on their own."""
+    from crowdsam_amd import hip
+    m, n, k = (1 << 21) + 37, 1040, 2048
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes = torch.randint(0, 126, (m, 2048), dtype=torch.uint8, device=cuda, generator=g)
+    scales = torch.full((16, m, 4), 120, dtype=torch.uint8, device=cuda)
+    qa = hip.MxTensor(codes, scales, "fp8", k)
+    qw = hip.mx_quantize(torch.randn(n, k, device=cuda, generator=g), "fp4")
+    out = hip.mx_gemm(qa, qw, out_dtype=torch.bfloat16)
+    assert m * n > 1 << 31 and codes.numel() > 1 << 32
+    assert torch.equal(out[-130:], hip.mx_gemm(qa.rows(m - 130, m), qw, out_dtype=torch.bfloat16))
+    assert torch.equal(out[:130], hip.mx_gemm(qa.rows(0, 130), qw, out_dtype=torch.bfloat16))
+
+
+def test_streams_and_graph_replays(cuda):
+    """The four operators as a run on a stream of their own and captured; each replay is checked against the eager result."""
+    from crowdsam_amd import hip
+    g = gen(3)
+    x = torch.randn(150, 256, generator=g).half().to(cuda)
+    r = torch.randn(150, 256, generator=g).to(cuda)
+    gamma = torch.rand(256, generator=g).to(cuda)
+    w = hip.mx_quantize(torch.randn(192, 256, generator=g).to(cuda), "fp4")
+
+    def step():
+        y, h = hip.rms_norm(x, gamma, 1e-6, residual=r, out_dtype="fp8")
+        c = hip.mx_gemm(y, w, act=hip.ACT_GELU)
+        return h, c, hip.mx_dequantize(hip.mx_quantize(c, "fp4"), out_dtype=torch.float16)
+
+    want = [t.clone() for t in step()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step()
+        again = step()
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b, c in zip(want, got, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        x.mul_(0.5 if i % 2 else 2.0)
+        r.add_(0.25)
+        fresh = [t.clone() for t in step()]
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, fresh):
+            assert torch.equal(a, b)
+
+
+def test_runs_are_bitwise_repeatable(cuda):
+    from crowdsam_amd import hip
+    for m in (3, 50, 400):
+        a, w = operands(m, 300, 1024, "fp8", m)
+        qa, qw = hip.mx_quantize(a.to(cuda), "fp8"), hip.mx_quantize(w.to(cuda), "fp4")
+        first = hip.mx_gemm(qa, qw, out_dtype=torch.float32)
+        for _ in range(5):
+            assert torch.equal(first, hip.mx_gemm(qa, qw, out_dtype=torch.float32))
