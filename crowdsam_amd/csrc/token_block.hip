@@ -74,10 +74,13 @@ __device__ __forceinline__ floatx4 ln_row(const float* y, const float* __restric
   const float s = v[0] + v[1] + v[2] + v[3];
   const float mean = csam_wave_sum(s) / 256.f;
   float q = 0.f;
+  {                                          // product and sum rounded apart, as csam_layernorm_cast's are: left to itself the compiler
+#pragma clang fp contract(off)               // contracts them in one kernel and not in the other
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float d = v[e] - mean;
-    q += d * d;
+    for (int e = 0; e < 4; ++e) {
+      const float d = v[e] - mean;
+      q += d * d;
+    }
   }
   const float rstd = rsqrtf(csam_wave_sum(q) / 256.f + eps);
   const floatx4 g = *(const floatx4*)(gamma + lane * 4);
