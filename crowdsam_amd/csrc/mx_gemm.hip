@@ -5,7 +5,13 @@
 // blocks is free as long as A and W agree: instruction kk of a 128-wide step takes blocks kk and 2 + kk, so that a lane's two
 // instructions read neighbouring blocks 2g, 2g + 1 and its two scale bytes are one aligned 16-bit load.  An E4M3 operand is spread
 // differently: lane group g holds halves g (16 codes) of BOTH blocks.
+// What the instruction keeps: E2M1 products are summed as fp32 sums them.  With an E4M3 operand it lines 16 neighbouring products up to
+// the largest and drops bits below 2^-13 of that (measured: a product 2^-14 of its neighbour vanishes, one in the next 16 does not); on
+// gaussian rows the result is 4.5e-6 off in norm, against the 2e-2 that rounding the operand to E4M3 cost.  Taking the 16 apart would
+// double the instructions.
 // W rows are the instruction's row operand, A rows its columns: a lane ends up with 4 consecutive n of one row m.
+#include <type_traits>
+#include <utility>
 #include "mx_common.h"
 
 namespace {
@@ -23,9 +29,23 @@ struct MxGemmArgs {
 typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 __device__ __forceinline__ void glds16(const void* g, void* l) { __builtin_amdgcn_global_load_lds((gptr_t)g, (lptr_t)l, 16, 0, 0); }
+__device__ __forceinline__ void glds4(const void* g, void* l) { __builtin_amdgcn_global_load_lds((gptr_t)g, (lptr_t)l, 4, 0, 0); }
 
 __device__ __forceinline__ float mx_elem(const void* p, int dt, long i) {
   return dt == CSAM_DT_F32 ? ((const float*)p)[i] : dt == CSAM_DT_F16 ? (float)((const half_t*)p)[i] : (float)((const bf16_t*)p)[i];
+}
+
+// GELU, as csam_gemm_f16 computes it: the erf form where the result stays fp32, for 16-bit results the polynomial of Phi (off by 6.5e-5 at
+// most, 12 instructions where erf takes 14 and two of quarter rate; a product with K = 1024 spends as long here as in its matrix
+// instructions)
+__device__ __forceinline__ void mx_gelu4(floatx4& v, int c_dt) {
+  if (c_dt == CSAM_DT_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = csam_gelu_erf(v[i]);
+  } else {
+    const float2_t a = csam_gelu_poly2(float2_t{v[0], v[1]}), b = csam_gelu_poly2(float2_t{v[2], v[3]});
+    v = floatx4{a[0], a[1], b[0], b[1]};
+  }
 }
 
 // 4 consecutive columns n .. n + 3 of row m: bias, activation, residual, rounding, store
@@ -39,10 +59,8 @@ __device__ __forceinline__ void mx_epilogue4(const MxGemmArgs& p, int m, int n, 
       for (int i = 0; i < 4; ++i)
         if (n + i < p.N) v[i] += p.bias[n + i];
   }
-  if (p.act != CSAM_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = csam_apply_act(v[i], p.act);
-  }
+  if (p.act == CSAM_ACT_GELU) mx_gelu4(v, p.c_dt);
+  else if (p.act == CSAM_ACT_RELU) v = floatx4{fmaxf(v[0], 0.f), fmaxf(v[1], 0.f), fmaxf(v[2], 0.f), fmaxf(v[3], 0.f)};
   if (full) {
     if (p.R) {
       const long at = (long)m * p.ldr + n;
@@ -77,6 +95,60 @@ __device__ __forceinline__ void mx_epilogue4(const MxGemmArgs& p, int m, int n, 
   }
 }
 
+// 4 consecutive columns of B rows STEP apart, all four inside N or none; every choice is uniform and made once for the B rows
+template <int B, int STEP>
+__device__ __forceinline__ void mx_epilogue_rows(const MxGemmArgs& p, int m, int n, floatx4 bz, floatx4 (&v)[B]) {
+  typedef bf16_t bf16x4_t __attribute__((ext_vector_type(4)));
+  if (n >= p.N) return;
+  floatx4 res[B];
+  if (p.R) {
+    const long at = (long)m * p.ldr + n;
+    if (p.r_dt == CSAM_DT_F32) {
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (m + b * STEP < p.M) res[b] = *(const floatx4*)((const float*)p.R + at + (long)b * STEP * p.ldr);
+    } else {
+      uintx2 u[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (m + b * STEP < p.M) u[b] = *(const uintx2*)((const half_t*)p.R + at + (long)b * STEP * p.ldr);
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (p.r_dt == CSAM_DT_F16) {
+          const half4_t h = __builtin_bit_cast(half4_t, u[b]);
+          res[b] = floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+        } else {
+          res[b] = floatx4{csam_lo_bf16(u[b][0]), csam_hi_bf16(u[b][0]), csam_lo_bf16(u[b][1]), csam_hi_bf16(u[b][1])};
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < B; ++b) v[b] += bz;
+  if (p.act == CSAM_ACT_GELU) {
+#pragma unroll
+    for (int b = 0; b < B; ++b) mx_gelu4(v[b], p.c_dt);
+  } else if (p.act == CSAM_ACT_RELU) {
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[b][i] = v[b][i] > 0.f ? v[b][i] : 0.f;
+  }
+  if (p.R) {
+#pragma unroll
+    for (int b = 0; b < B; ++b) v[b] += res[b];
+  }
+  const long at = (long)m * p.ldc + n;
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    if (m + b * STEP >= p.M) return;
+    const long o = at + (long)b * STEP * p.ldc;
+    if (p.c_dt == CSAM_DT_F32) *(floatx4*)((float*)p.C + o) = v[b];
+    else if (p.c_dt == CSAM_DT_F16) *(half4_t*)((half_t*)p.C + o) = half4_t{(half_t)v[b][0], (half_t)v[b][1], (half_t)v[b][2], (half_t)v[b][3]};
+    else *(bf16x4_t*)((bf16_t*)p.C + o) = bf16x4_t{(bf16_t)v[b][0], (bf16_t)v[b][1], (bf16_t)v[b][2], (bf16_t)v[b][3]};
+  }
+}
+
 template <int FA, int KK>
 __device__ __forceinline__ floatx16 mx_mfma32(const intx8& w, const intx8& a, floatx16 c, int sw, int sa) {
   constexpr int AF = FA == CSAM_MX_FP8 ? 0 : 4;
@@ -97,53 +169,93 @@ __device__ __forceinline__ intx8 mx_frag(const void* lo, const void* hi) {
 }
 
 // --------------------------------------------------------------------------------------------------------------- tiled form
-// TM x TN tile, WGM x WGN waves of 32x32 MFMA tiles, 128-wide K steps through NS = 2 LDS stages filled by 16-byte LDS-DMA.
-// LDS lines of 128 bytes = one E4M3 row or two E2M1 rows of the step; slot ^= line & 7 on the DMA's source address and on the reads.
-template <int FA, int TM, int TN, int WGM, int WGN>
-__global__ __launch_bounds__(WGM * WGN * 64) void mx_gemm_kernel(MxGemmArgs p) {
-  constexpr int NW = WGM * WGN;
-  constexpr int RA = FA == CSAM_MX_FP8 ? 128 : 64, RW = 64;
-  constexpr int ABYTES = TM * RA, STAGE = ABYTES + TN * RW;
-  constexpr int LA = ABYTES / 1024 / NW, LW = TN * RW / 1024 / NW;
-  static_assert(LA * NW * 1024 == ABYTES && LW * NW * 1024 == TN * RW, "whole DMA instructions per wave");
-  constexpr int MI = TM / WGM / 32, NI = TN / WGN / 32;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+// TM x TN tile, WGM x WGN waves of 32x32 MFMA tiles, KS-wide steps through NS LDS stages filled by LDS-DMA (codes 16 bytes, scales 4
+// bytes per lane).  LDS lines are 128 bytes: a row of the step (256 E2M1 or 128 E4M3 codes), or two rows of 128 E2M1 codes.  The LDS reads
+// 256 bytes a cycle, sixteen lanes of 16 bytes: a row's pieces are turned by XOR with the index of its 256 bytes, on the DMA's source
+// address and on the reads, so that sixteen lanes reading one column of pieces meet no bank twice.
+template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS>
+struct MxTile {
+  static constexpr int NW = WGM * WGN;
+  static constexpr int RA = FA == CSAM_MX_FP8 ? KS : KS / 2, RW = KS / 2;                // bytes of a row per step
+  static constexpr int ABYTES = TM * RA, WBYTES = TN * RW, SBYTES = (TM + TN) * (KS / 32), STAGE = ABYTES + WBYTES + SBYTES;
+  static constexpr int RUNS = (TM + TN) / 64 * (KS / 128);                               // scale fetches of 64 rows x 4 bytes
+  static constexpr int LA = ABYTES / 1024 / NW, LW = WBYTES / 1024 / NW, LS = (RUNS + NW - 1) / NW;
+  static constexpr int PER = LA + LW + LS;               // DMA instructions of a wave per stage: what a counted wait leaves in flight
+  static constexpr int MI = TM / WGM / 32, NI = TN / WGN / 32;
+  static constexpr int EPI = NW * 32 * (NI * 32 + 4) * 4;    // a wave's 32 rows of fp32 results on their way out, row by row
+  static constexpr int LDS = NS * STAGE > EPI ? NS * STAGE : EPI;
+  static_assert(LA * NW * 1024 == ABYTES && LW * NW * 1024 == WBYTES && TM % 64 == 0 && TN % 64 == 0, "whole DMA instructions per wave");
+  static_assert((RA == 64 || RA == 128) && (RW == 64 || RW == 128), "line formats");
+};
+
+// tile of workgroup b: each XCD (b % 8) takes a contiguous run of the order, which walks GROUP tile rows column by column, so that the
+// workgroups an XCD runs at once share operand panels in its L2
+__device__ __forceinline__ void mx_tile_of(int b, int nm, int nn, int& tm, int& tn) {
+  constexpr int GROUP = 8;
+  const int n = nm * nn, x = b & 7, q = n >> 3, r = n & 7;
+  const int i = x * q + min(x, r) + (b >> 3);
+  const int per = GROUP * nn, grp = i / per, first = grp * GROUP, rows = min(GROUP, nm - first), j = i - grp * per;
+  tn = j / rows;
+  tm = first + j - tn * rows;
+}
+
+// byte of piece c (16 bytes) of row r in an operand whose rows are RB bytes
+template <int RB>
+__device__ __forceinline__ int mx_lds_piece(int r, int c) {
+  return RB == 128 ? r * 128 + ((c ^ ((r >> 1) & 7)) << 4) : r * 64 + ((c ^ ((r >> 2) & 3)) << 4);
+}
+
+template <int... I, typename F>
+__device__ __forceinline__ void mx_for_each(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F>
+__device__ __forceinline__ void mx_for(F f) { mx_for_each(std::make_integer_sequence<int, N>{}, f); }
+#define MX_C(x) (std::integral_constant<int, (x)>{})
+
+template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS>
+__global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 ? 1 : 2) void mx_gemm_kernel(MxGemmArgs p) {
+  using T = MxTile<FA, TM, TN, WGM, WGN, NS, KS>;
+  constexpr int NW = T::NW, RA = T::RA, RW = T::RW, LA = T::LA, LW = T::LW, LS = T::LS, MI = T::MI, NI = T::NI, NH = KS / 64;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int wm = wave / WGN, wn = wave % WGN;
-  const int tn_n = (p.N + TN - 1) / TN;
-  const int bm0 = (int)(blockIdx.x / tn_n) * TM, bn0 = (int)(blockIdx.x % tn_n) * TN;
+  int tm, tn;
+  mx_tile_of(blockIdx.x, (p.M + TM - 1) / TM, (p.N + TN - 1) / TN, tm, tn);
+  const int bm0 = tm * TM, bn0 = tn * TN;
 
-  // DMA sources: lane l of instruction i fills line i * 8 + l / 8, slot l % 8, which holds piece (l % 8) ^ (line & 7)
-  const int lg = (lane & 7) ^ (lane >> 3);
-  const uint8_t *asrc[LA], *wsrc[LW];
-#pragma unroll
-  for (int i = 0; i < LA; ++i) {
-    const int line = (wave * LA + i) * 8 + (lane >> 3);
-    const int row = RA == 128 ? line : 2 * line + (lg >> 2), c = RA == 128 ? lg : lg & 3;
-    asrc[i] = p.A + (long)min(bm0 + row, p.M - 1) * p.lda + c * 16;
-  }
-#pragma unroll
-  for (int i = 0; i < LW; ++i) {
-    const int line = (wave * LW + i) * 8 + (lane >> 3);
-    wsrc[i] = p.W + (long)min(bn0 + 2 * line + (lg >> 2), p.N - 1) * p.ldw + (lg & 3) * 16;
-  }
-  auto stage = [&](int slot, int t) {
-    uint8_t* base = smem + slot * STAGE;
-#pragma unroll
-    for (int i = 0; i < LA; ++i) glds16(asrc[i] + (long)t * RA, base + (wave * LA + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < LW; ++i) glds16(wsrc[i] + (long)t * RW, base + ABYTES + (wave * LW + i) * 1024);
+  // DMA sources (32-bit offsets from the tile's first row; rows behind the last one are the last one again and never stored): lane l of
+  // instruction i fills byte i * 1024 + l * 16, i.e. it fetches the piece that belongs there
+  const uint8_t* abase = p.A + (long)bm0 * p.lda;
+  const uint8_t* wbase = p.W + (long)bn0 * p.ldw;
+  unsigned aoff[LA], woff[LW], soff[LS];
+  const uint8_t* sbase[LS];
+  long sstep[LS];
+  int sdst[LS];
+  auto source = [&](int at, int rb, int rows, unsigned ld) {        // piece at byte `at` of an operand's stage
+    const int row = at / rb, c = (at % rb) >> 4, turned = rb == 128 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3);
+    return (unsigned)min(row, rows - 1) * ld + turned * 16;
   };
-
-  // fragment addresses within a stage (tile i, instruction kk): + i * 32 rows, ^ by kk
-  const int r = lane & 31, g = lane >> 5;
-  const int off64 = (r >> 1) * 128 + (((((r & 1) << 2) + 2 * g) ^ ((r >> 1) & 7)) << 4);       // E2M1: piece 2g + kk of the row
-  const int off128 = r * 128 + ((g ^ (r & 7)) << 4);                                          // E4M3: pieces 2 kk + g and 4 + 2 kk + g
-  const uint8_t *sap[MI], *swp[NI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) sap[i] = p.As + (long)min(bm0 + (wm * MI + i) * 32 + r, p.M - 1) * 4 + 2 * g;
+  for (int i = 0; i < LA; ++i) aoff[i] = source((wave * LA + i) * 1024 + lane * 16, RA, p.M - bm0, (unsigned)p.lda);
 #pragma unroll
-  for (int j = 0; j < NI; ++j) swp[j] = p.Ws + (long)min(bn0 + (wn * NI + j) * 32 + r, p.N - 1) * 4 + 2 * g;
+  for (int i = 0; i < LW; ++i) woff[i] = source((wave * LW + i) * 1024 + lane * 16, RW, p.N - bn0, (unsigned)p.ldw);
+#pragma unroll
+  for (int i = 0; i < LS; ++i) {                          // a wave without a run of its own repeats the last one
+    const int run = min(wave * LS + i, T::RUNS - 1), h = run / ((TM + TN) / 64), at = run % ((TM + TN) / 64);
+    const bool isa = at < TM / 64;
+    const int row = (isa ? at : at - TM / 64) * 64 + lane;
+    sstep[i] = isa ? p.a_ss : p.w_ss;
+    sbase[i] = (isa ? p.As + (long)bm0 * 4 : p.Ws + (long)bn0 * 4) + h * sstep[i];
+    soff[i] = (unsigned)min(row, isa ? p.M - 1 - bm0 : p.N - 1 - bn0) * 4u;
+    sdst[i] = T::ABYTES + T::WBYTES + run * 256;
+  }
+  // DMA instruction d of stage t (its source; a step behind the last one is the last one again) into stage `slot`
+  auto dma = [&](auto d_, int slot, int t) {
+    constexpr int d = decltype(d_)::value;
+    uint8_t* base = smem + slot * T::STAGE;
+    if constexpr (d < LA) glds16(abase + (long)t * RA + aoff[d], base + (wave * LA + d) * 1024);
+    else if constexpr (d < LA + LW) glds16(wbase + (long)t * RW + woff[d - LA], base + T::ABYTES + (wave * LW + d - LA) * 1024);
+    else glds4(sbase[d - LA - LW] + (long)t * (KS / 128) * sstep[d - LA - LW] + soff[d - LA - LW], base + sdst[d - LA - LW]);
+  };
 
   floatx16 acc[MI][NI];
 #pragma unroll
@@ -153,59 +265,125 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mx_gemm_kernel(MxGemmArgs p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  const int nt = p.Kp / 128;
-  int sa[MI], sw[NI];
-  stage(0, 0);
+  // The main loop issues one stream per wave, in the order written here: part h of a step is MI * NI matrix instructions, and between them
+  // go the LDS reads of the next part (a second fragment set) and a share of a later stage's DMA.  In a bunch behind the barrier the
+  // DMAs of all waves queue for the one address unit of the CU while the matrix pipes wait.
+  //   last part of step t:    reads of step t + 1's part 0; the first DMAs of step t + NS into stage t, which is read out
+  //   other parts of step t:  reads of the next part; the rest of step t + NS - 1
+  // Before the last part a wait and a barrier publish step t + 1: of the DMAs issued so far, steps t + 2 .. t + NS - 1 stay in flight.
+  const int nt = p.Kp / KS;
+  const int r = lane & 31, g = lane >> 5;
+  constexpr int NQ = MI * NI, FR = FA == CSAM_MX_FP8 ? 2 : 1, NF = NI + MI * FR, NSC = MI + NI, PER = T::PER;
+  intx8 af[2][MI], wf[2][NI];
+  int sa[2][MI], sw[2][NI];                               // two bytes each: the scales of parts 2h and 2h + 1
+  // LDS read k of part h: W fragments, A fragments (E4M3: two reads each); and scale read k of parts h and h + 1
+  auto read = [&](auto k_, auto h_, int slot) {
+    constexpr int k = decltype(k_)::value, h = decltype(h_)::value, set = h & 1;
+    constexpr int c = (h >> 1) * 4 + (h & 1);                                               // E2M1: piece c + 2g of the row
+    const uint8_t* base = smem + slot * T::STAGE;
+    if constexpr (k < NI) {
+      const uintx4 v = *(const uintx4*)(base + T::ABYTES + (wn * NI + k) * 32 * RW + mx_lds_piece<RW>(r, c + 2 * g));
 #pragma unroll
-  for (int i = 0; i < MI; ++i) sa[i] = *(const unsigned short*)sap[i];
+      for (int e = 0; e < 4; ++e) wf[set][k][e] = (int)v[e];
+    } else {
+      constexpr int i = (k - NI) / FR, f = (k - NI) % FR;
+      const int pc = FA == CSAM_MX_FP8 ? 4 * f + 2 * h + g : c + 2 * g;                        // E4M3: pieces 2h + g and 4 + 2h + g
+      const uintx4 v = *(const uintx4*)(base + (wm * MI + i) * 32 * RA + mx_lds_piece<RA>(r, pc));
 #pragma unroll
-  for (int j = 0; j < NI; ++j) sw[j] = *(const unsigned short*)swp[j];
-  for (int t = 0; t < nt; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's share of step t has landed
-    __builtin_amdgcn_s_barrier();                          // ... and everybody's; step t - 1's stage is read out
+      for (int e = 0; e < 4; ++e) af[set][i][4 * f + e] = (int)v[e];
+    }
+  };
+  auto read_scale = [&](auto k_, auto h_, auto ss_, int slot) {
+    constexpr int k = decltype(k_)::value, h = decltype(h_)::value, ss = decltype(ss_)::value;
+    const uint8_t* sb = smem + slot * T::STAGE + T::ABYTES + T::WBYTES + (h >> 1) * (TM + TN) * 4 + r * 4 + 2 * g;
+    if constexpr (k < MI) sa[ss][k] = *(const unsigned short*)(sb + (wm * MI + k) * 128);
+    else sw[ss][k - MI] = *(const unsigned short*)(sb + TM * 4 + (wn * NI + k - MI) * 128);
+  };
+  // part h: matrix instructions on scale set ss; between them the reads of part rh (scale set rs) from stage rslot and the DMAs
+  // [d0, d1) of step dt into stage dslot.  The reads go first, so that they are done when the part is.
+  auto part = [&](auto h_, auto ss_, auto rh_, auto rs_, int rslot, auto d0_, auto d1_, int dslot, int dt) {
+    constexpr int h = decltype(h_)::value, ss = decltype(ss_)::value, rh = decltype(rh_)::value;
+    constexpr int d0 = decltype(d0_)::value, d1 = decltype(d1_)::value;
+    constexpr int S = (rh & 1) == 0 ? NSC : 0, NR = NF + S, ND = d1 - d0;
+    constexpr int GAPS = NQ < 4 ? NQ : 4, RPG = (NR + GAPS - 1) / GAPS, G0 = NQ > 4 ? 2 : 0;
+    mx_for<NQ>([&](auto q_) {
+      constexpr int q = decltype(q_)::value, i = q / NI, j = q % NI;
+      acc[i][j] = mx_mfma32<FA, (h & 1)>(wf[h & 1][j], af[h & 1][i], acc[i][j], sw[ss][j], sa[ss][i]);
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int r0 = q * RPG < NR ? q * RPG : NR, r1 = (q + 1) * RPG < NR ? (q + 1) * RPG : NR;
+      constexpr int e0 = q < G0 ? 0 : (q - G0) * ND / (NQ - G0), e1 = q < G0 ? 0 : (q - G0 + 1) * ND / (NQ - G0);
+      mx_for<r1 - r0>([&](auto x_) {
+        constexpr int k = r0 + decltype(x_)::value;
+        if constexpr (k < S) read_scale(MX_C(k), rh_, rs_, rslot);
+        else read(MX_C(k - S), rh_, rslot);
+      });
+      mx_for<e1 - e0>([&](auto x_) { dma(MX_C(d0 + e0 + decltype(x_)::value), dslot, dt); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  constexpr int FIRST = (PER + NH - 1) / NH;              // DMAs of a stage that its first (the last) part issues
+  mx_for<NS - 1>([&](auto s_) { mx_for<PER>([&](auto d_) { dma(d_, decltype(s_)::value, min(decltype(s_)::value, nt - 1)); }); });
+  mx_for<FIRST>([&](auto d_) { dma(d_, NS - 1, min(NS - 1, nt - 1)); });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * PER + FIRST) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  mx_for<NSC>([&](auto k_) { read_scale(k_, MX_C(0), MX_C(0), 0); });
+  mx_for<NF>([&](auto k_) { read(k_, MX_C(0), 0); });
+  // step t, t % UN = u: stages and scale sets are constants of the unrolled loop.  Scale sets: by step (NH = 2) or by pair of parts.
+  constexpr int UN = NH == 2 && NS % 2 ? 2 * NS : NS;
+  auto step = [&](int t, auto u_) {
+    constexpr int u = decltype(u_)::value, slot = u % NS, next = (u + 1) % NS, prev = (u + NS - 1) % NS, us = u & 1;
+    mx_for<NH - 1>([&](auto h_) {
+      constexpr int h = decltype(h_)::value;
+      constexpr int d0 = FIRST + h * (PER - FIRST) / (NH - 1), d1 = FIRST + (h + 1) * (PER - FIRST) / (NH - 1);
+      part(h_, MX_C(NH == 2 ? us : (h >> 1) & 1), MX_C(h + 1), MX_C(((h + 1) >> 1) & 1), slot, MX_C(d0), MX_C(d1), prev, min(t + NS - 1, nt - 1));
+    });
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * PER) : "memory");
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    int na[MI], nw[NI];
-    if (t + 1 < nt) {
-      stage((t + 1) & 1, t + 1);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) na[i] = *(const unsigned short*)(sap[i] + (long)(t + 1) * p.a_ss);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) nw[j] = *(const unsigned short*)(swp[j] + (long)(t + 1) * p.w_ss);
-    }
-    const uint8_t* ab = smem + (t & 1) * STAGE + wm * MI * 32 * RA;
-    const uint8_t* wb = smem + (t & 1) * STAGE + ABYTES + wn * NI * 32 * RW;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      intx8 af[MI], wf[NI];
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        if constexpr (RA == 128) af[i] = mx_frag(ab + i * 4096 + (off128 ^ (kk << 5)), ab + i * 4096 + (off128 ^ (kk << 5) ^ 64));
-        else af[i] = mx_frag(ab + i * 2048 + (off64 ^ (kk << 4)));
+    part(MX_C(NH - 1), MX_C(NH == 2 ? us : 1), MX_C(0), MX_C(NH == 2 ? us ^ 1 : 0), next, MX_C(0), MX_C(FIRST), slot, min(t + NS, nt - 1));
+  };
+  for (int t = 0;;) {
+    bool more = true;
+    mx_for<UN>([&](auto u_) {
+      if (more) {
+        step(t, u_);
+        more = ++t < nt;
       }
-#pragma unroll
-      for (int j = 0; j < NI; ++j) wf[j] = mx_frag(wb + j * 2048 + (off64 ^ (kk << 4)));
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-          acc[i][j] = kk ? mx_mfma32<FA, 1>(wf[j], af[i], acc[i][j], sw[j], sa[i]) : mx_mfma32<FA, 0>(wf[j], af[i], acc[i][j], sw[j], sa[i]);
-    }
-    if (t + 1 < nt) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i) sa[i] = na[i];
-#pragma unroll
-      for (int j = 0; j < NI; ++j) sw[j] = nw[j];
-    }
+    });
+    if (!more) break;
   }
+
+  // Epilogue: a wave passes its results 32 rows at a time through LDS of its own and takes them out row by row, so that NI * 32
+  // consecutive columns of a row move together (straight from the registers a store would touch 32 rows with 32 bytes each).
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");    // the repeated fetches have landed
+  __builtin_amdgcn_s_barrier();                                 // ... everybody's, and every stage is read out
+  asm volatile("" ::: "memory");
+  constexpr int COLS = NI * 32, PITCH = COLS + 4;          // + 4 floats: rows start 4 banks apart
+  constexpr int LPR = COLS / 4, RPI = 64 / LPR, B = 4;     // lanes of a row, rows of an access, accesses of a batch
+  float* buf = (float*)smem + wave * 32 * PITCH;
+  const int n = bn0 + wn * COLS + (lane % LPR) * 4, mr = bm0 + wm * MI * 32 + lane / LPR;
+  const floatx4 bz = p.vec && p.bias && n < p.N ? *(const floatx4*)(p.bias + n) : floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int m = bm0 + (wm * MI + i) * 32 + r;
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n = bn0 + (wn * NI + j) * 32 + 4 * g;
+    for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        mx_epilogue4(p, m, n + 8 * e, floatx4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]});
+        *(floatx4*)(buf + r * PITCH + j * 32 + 8 * e + 4 * g) =
+            floatx4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+    const float* src = buf + lane / LPR * PITCH + (lane % LPR) * 4;
+    if (p.vec) {                                           // N is a multiple of 4: a lane's four columns are inside or outside together
+#pragma unroll 1
+      for (int s = 0; s < 32 / RPI; s += B) {
+        floatx4 v[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) v[b] = *(const floatx4*)(src + (s + b) * RPI * PITCH);
+        mx_epilogue_rows<B, RPI>(p, mr + i * 32 + s * RPI, n, bz, v);
+      }
+    } else {
+#pragma unroll 1
+      for (int s = 0; s < 32 / RPI; ++s) mx_epilogue4(p, mr + i * 32 + s * RPI, n, *(const floatx4*)(src + s * RPI * PITCH));
     }
   }
 }
@@ -266,20 +444,44 @@ __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(MxGemmArgs p) {
   }
 }
 
-template <int FA>
-int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
-  const long tn16 = csam_cdiv(p.N, 16);
-  if (p.M <= 64) {
-    if (p.M <= 16) mx_gemm_rows_kernel<FA, 1, 4><<<(unsigned)tn16, 256, 0, st>>>(p);
-    else if (p.M <= 32) mx_gemm_rows_kernel<FA, 2, 4><<<(unsigned)tn16, 256, 0, st>>>(p);
-    else mx_gemm_rows_kernel<FA, 4, 4><<<(unsigned)tn16, 256, 0, st>>>(p);
-  } else {
-    const long grid = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128);
-    CSAM_REQUIRE(grid < (1L << 31), "csam_mx_gemm: too many tiles");
-    mx_gemm_kernel<FA, 128, 128, 2, 2><<<(unsigned)grid, 256, 0, st>>>(p);
-  }
+template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS>
+int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
+  const long grid = (long)csam_cdiv(p.M, TM) * csam_cdiv(p.N, TN);
+  CSAM_REQUIRE(grid < (1L << 31), "csam_mx_gemm: too many tiles");
+  mx_gemm_kernel<FA, TM, TN, WGM, WGN, NS, KS><<<(unsigned)grid, WGM * WGN * 64, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_mx_gemm");
   return CSAM_OK;
+}
+
+// Which form: the largest tile that still fills the chip, since the products move their operands L2 -> LDS at 7 to 9 TB/s and are bound by
+// that before the matrix units; us on one MI355X (M x N x K, fp16 out, no epilogue), E2M1 / E4M3 activations:
+//   rows      against 64x64      32 x 4096 x 4096:    5.8 / 7.7    against  7.0 / 9.9      64 x 4096 x 4096: 8.1 / 11.8 against 7.0 / 9.2
+//   64x64     against 128 wide   512 x 4096 x 4096:   10.8 / 14.7  against 17.0 / 22.1
+//   128 wide  against 64x64      2048 x 4096 x 4096:  26.0 / 31.8  against 33.4 / 50.1     (E4M3: 128x256 tiles, eight waves)
+//   256x256   against 128 wide   4096 x 4096 x 4096:  42.0 / 55.1  against 47.8 / 60.4     2048 x 4096: 34.0 / 45.8 against 26.0 / 31.8
+//   a part-filled last round of 256x256 tiles (5330 x 4096 x 1024, 1.3 rounds): 31.4 / 38.7 against 30.3 / 32.2 with 128x128
+template <int FA>
+int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
+  const long t16 = (long)csam_cdiv(p.M, 16) * csam_cdiv(p.N, 16);
+  if (p.M <= 16 || t16 <= 512) {
+    if (t16 <= 256 || p.M <= 16) mx_gemm_rows_kernel<FA, 1, 4><<<(unsigned)t16, 256, 0, st>>>(p);
+    else mx_gemm_rows_kernel<FA, 2, 4><<<(unsigned)((long)csam_cdiv(p.M, 32) * csam_cdiv(p.N, 16)), 256, 0, st>>>(p);
+    CSAM_LAUNCH_CHECK("csam_mx_gemm");
+    return CSAM_OK;
+  }
+  const long t256 = (long)csam_cdiv(p.M, 256) * csam_cdiv(p.N, 256), rounds = (t256 + 255) / 256;
+  const bool filled = rounds >= 4 || t256 * 4 >= rounds * 256 * 3;
+  if constexpr (FA == CSAM_MX_FP4) {
+    if (filled) return mx_tiles<FA, 256, 256, 2, 4, 3, 128>(st, p);
+    if ((long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128) >= 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 256>(st, p);
+    return mx_tiles<FA, 64, 64, 2, 2, 3, 256>(st, p);
+  } else {
+    if (filled) return mx_tiles<FA, 256, 256, 4, 2, 3, 128>(st, p);
+    const long t128 = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 256);
+    if (t128 > 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 128>(st, p);
+    if (t128 >= 128) return mx_tiles<FA, 128, 256, 2, 4, 3, 128>(st, p);
+    return mx_tiles<FA, 64, 64, 2, 2, 3, 128>(st, p);
+  }
 }
 
 }  // namespace
@@ -298,12 +500,13 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
   CSAM_REQUIRE(dt_ok(c_dtype) && (!residual || dt_ok(r_dtype)), "csam_mx_gemm: bad dtype");
   CSAM_REQUIRE(act == CSAM_ACT_NONE || act == CSAM_ACT_GELU || act == CSAM_ACT_RELU, "csam_mx_gemm: bad activation %d", act);
   CSAM_REQUIRE(lda >= (a_fmt == CSAM_MX_FP8 ? Kp : Kp / 2) && ldw >= Kp / 2, "csam_mx_gemm: code rows are shorter than %d padded columns", Kp);
+  CSAM_REQUIRE(lda < (1 << 24) && ldw < (1 << 24), "csam_mx_gemm: code rows 16 MB apart or more");
   CSAM_REQUIRE(al(A, lda, 16) && al(W, ldw, 16), "csam_mx_gemm: codes and their row pitch have to be multiples of 16 bytes");
   CSAM_REQUIRE(al(A_scales, a_scale_stride, 4) && al(W_scales, w_scale_stride, 4) && a_scale_stride >= 4L * M && w_scale_stride >= 4L * N,
                "csam_mx_gemm: scale groups have to lie 4-byte aligned, at least 4 * rows bytes apart");
   CSAM_REQUIRE(ldc >= N && (!residual || ldr >= N), "csam_mx_gemm: an output row pitch is shorter than N");
   auto es = [](int dt) { return dt == CSAM_DT_F32 ? 4 : 2; };
-  const int vec = al(C, ldc * es(c_dtype), 4 * es(c_dtype)) && (!residual || al(residual, ldr * es(r_dtype), 4 * es(r_dtype))) &&
+  const int vec = N % 4 == 0 && al(C, ldc * es(c_dtype), 4 * es(c_dtype)) && (!residual || al(residual, ldr * es(r_dtype), 4 * es(r_dtype))) &&
                   (!bias || (uintptr_t)bias % 16 == 0);
   MxGemmArgs p = {(const uint8_t*)A, lda, (const uint8_t*)A_scales, a_scale_stride, (const uint8_t*)W, ldw, (const uint8_t*)W_scales,
                   w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act, M, N, Kp, vec};

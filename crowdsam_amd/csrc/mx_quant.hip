@@ -82,7 +82,7 @@ struct RmsArgs {
   float eps;
   void* y; long ldy; int y_kind;          // CSAM_DT_*, or RMS_MX + CSAM_MX_*
   uint8_t* scales; long sstride;
-  int M, D, Dp, vec, rows;                // rows: rows of a row slot (a wave when NW = 1, the workgroup otherwise)
+  int M, D, Dp, vec, gvec, rows;          // rows: rows of a row slot (a wave when NW = 1, the workgroup otherwise)
 };
 constexpr int RMS_MX = 16;
 
@@ -101,7 +101,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsAr
 #pragma unroll
   for (int j = 0; j < MAXC; ++j) {
     const int k = (c0 + j * STEP) * 8;
-    csam_load8_tail(p.gamma + k, D - k, g[j]);
+    if (k + 8 <= D && p.gvec) csam_load8(p.gamma + k, g[j]);
+    else csam_load8_tail(p.gamma + k, D - k, g[j]);
   }
   const float inv_d = 1.0f / (float)D;
   for (int i = 0; i < p.rows; ++i) {
@@ -177,12 +178,14 @@ int rms_launch(hipStream_t st, RmsArgs& p) {
 #define RMS_GO(NW, MAXC)                                                                              \
   do {                                                                                                \
     const int slots = NW == 1 ? 4 : 1;                                                                \
-    p.rows = 1;                                                                                       \
+    p.rows = max(1, min(16, p.M / (4096 / NW)));                                                      \
     rms_norm_kernel<T, RK, NW, MAXC><<<csam_cdiv(p.M, (long)slots * p.rows), NW == 1 ? 256 : NW * 64, 0, st>>>(p); \
   } while (0)
   if (chunks <= 64) RMS_GO(1, 1);
   else if (chunks <= 128) RMS_GO(1, 2);
+  else if (chunks <= 192) RMS_GO(1, 3);
   else if (chunks <= 256) RMS_GO(1, 4);
+  else if (chunks <= 512) RMS_GO(4, 2);
   else if (chunks <= 1024) RMS_GO(4, 4);
   else RMS_GO(16, 4);
 #undef RMS_GO
@@ -276,6 +279,7 @@ static int rms_any(hipStream_t st, RmsArgs& p, int x_dtype, int r_dtype, const c
   p.vec = aligned(p.x, p.ldx * dt_bytes(x_dtype), 16) &&
           (!p.r || (aligned(p.r, p.ldr * dt_bytes(r_dtype), 16) && aligned(p.h, p.ldh * dt_bytes(r_dtype), 16)));
   if (p.y_kind < RMS_MX) p.vec = p.vec && aligned(p.y, p.ldy * dt_bytes(p.y_kind), 16);
+  p.gvec = (uintptr_t)p.gamma % 16 == 0;
   const int rk = !p.r ? 0 : (r_dtype == CSAM_DT_F32 && x_dtype != CSAM_DT_F32) ? 2 : 1;
 #define GO(T) return rk == 0 ? rms_launch<T, 0>(st, p) : rk == 1 ? rms_launch<T, 1>(st, p) : rms_launch<T, 2>(st, p)
   if (x_dtype == CSAM_DT_F16) GO(half_t);
@@ -288,7 +292,7 @@ int csam_rms_norm(void* stream, const void* x, long ldx, int x_dtype, const void
                   const float* gamma, float eps, void* y, long ldy, int y_dtype, int M, int D) {
   if (M == 0) return CSAM_OK;
   CSAM_REQUIRE(dt_ok(y_dtype) && ldy >= D, "csam_rms_norm: bad output dtype %d or row pitch %ld", y_dtype, ldy);
-  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0, 0, 1};
+  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0, 0, 0, 1};
   return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm");
 }
 
@@ -298,7 +302,7 @@ int csam_rms_norm_mx(void* stream, const void* x, long ldx, int x_dtype, const v
   CSAM_REQUIRE(D > 0, "csam_rms_norm_mx: bad width %d", D);
   if (int rc = mx_check("csam_rms_norm_mx", codes, ldcodes, scales, scale_stride, fmt, M, D)) return rc;
   RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, codes, ldcodes, RMS_MX + fmt, (uint8_t*)scales, scale_stride, M, D,
-               csam_cdiv(D, 256) * 256, 0, 1};
+               csam_cdiv(D, 256) * 256, 0, 0, 1};
   return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm_mx");
 }
 

@@ -1176,10 +1176,13 @@ def coco_rle_string(counts):
 
 # ----------------------------------------------------------------------------------------------
 # microscaled (MX) operands, RMS norm, rotary positions.  These take fp16, bfloat16 and fp32 tensors on any HIP device, work on the
-# current stream of that device, allocate nothing but their outputs, and raise ValueError for arguments they do not take.
+# current stream of that device, allocate nothing but their outputs, and raise ValueError for arguments they do not take.  A call of one
+# token is bound by what happens here before the launch, so every attribute of a tensor is fetched once and messages are only built
+# where they are raised.
 # ----------------------------------------------------------------------------------------------
 _DT3 = {torch.float16: DT_F16, torch.float32: DT_F32, torch.bfloat16: 2}
 _MX = {"fp4": 0, "fp8": 1}
+_INT_MAX = (1 << 31) - 1
 
 
 class MxTensor(NamedTuple):
@@ -1196,83 +1199,104 @@ class MxTensor(NamedTuple):
         return MxTensor(self.codes[i:j], self.scales[:, i:j], self.fmt, self.K)
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
-
-
-def _mx_padded(K):
-    return -(-K // 256) * 256
-
-
-def _mx_empty(rows, K, fmt, device):
-    Kp = _mx_padded(K)
-    return MxTensor(torch.empty((rows, Kp // 2 if fmt == "fp4" else Kp), dtype=torch.uint8, device=device),
-                    torch.empty((Kp // 128, rows, 4), dtype=torch.uint8, device=device), fmt, K)
+def _mx_empty(like, rows, K, fmt):
+    Kp = -(-K // 256) * 256
+    return MxTensor(like.new_empty((rows, Kp // 2 if fmt == "fp4" else Kp), dtype=torch.uint8),
+                    like.new_empty((Kp // 128, rows, 4), dtype=torch.uint8), fmt, K)
 
 
 def _mx_check(q, who, name):
-    """(code row pitch, scale group pitch) of an operand whose shapes, dtypes and strides are what the kernels read."""
-    c, s = q.codes, q.scales
-    _need(q.fmt in _MX, f"{who}: {name} has format {q.fmt!r}, not 'fp4' or 'fp8'")
-    _need(q.K > 0, f"{who}: {name} has K = {q.K}")
-    Kp = _mx_padded(q.K)
-    _need(c.dtype == torch.uint8 and s.dtype == torch.uint8, f"{who}: {name} has {c.dtype} codes and {s.dtype} scales, not uint8")
-    _need(c.dim() == 2 and c.shape[1] == (Kp // 2 if q.fmt == "fp4" else Kp),
-          f"{who}: {name} has codes of shape {tuple(c.shape)}, not [rows, {Kp // 2 if q.fmt == 'fp4' else Kp}] (K = {q.K} padded to {Kp})")
-    rows = c.shape[0]
-    _need(tuple(s.shape) == (Kp // 128, rows, 4), f"{who}: {name} has scales of shape {tuple(s.shape)}, not {(Kp // 128, rows, 4)}")
-    ldc = c.stride(0) if rows > 1 else c.shape[1]
-    ss = s.stride(0) if Kp > 128 else 4 * rows
-    _need(rows == 0 or (c.stride(1) == 1 and ldc >= c.shape[1] and ldc % 16 == 0 and c.data_ptr() % 16 == 0),
-          f"{who}: {name} has code rows that are not contiguous, or not 16-byte aligned")
-    _need(rows == 0 or (s.stride(2) == 1 and (rows == 1 or s.stride(1) == 4) and ss >= 4 * rows and ss % 4 == 0 and s.data_ptr() % 4 == 0),
-          f"{who}: {name} has scales whose rows of a group are not 4 bytes apart")
-    return ldc, ss
+    """(rows, code row pitch, scale group pitch, code pointer, scale pointer) of an operand whose shapes, types and strides are what the
+    kernels read."""
+    c, s, fmt, K = q
+    if fmt not in _MX:
+        raise ValueError(f"{who}: {name} has format {fmt!r}, not 'fp4' or 'fp8'")
+    if not 0 < K <= _INT_MAX - 255:
+        raise ValueError(f"{who}: {name} has K = {K}")
+    Kp = -(-K // 256) * 256
+    width = Kp // 2 if fmt == "fp4" else Kp
+    if c.dtype != torch.uint8 or s.dtype != torch.uint8:
+        raise ValueError(f"{who}: {name} has {c.dtype} codes and {s.dtype} scales, not uint8")
+    shape = c.shape
+    if len(shape) != 2 or shape[1] != width or shape[0] > _INT_MAX:
+        raise ValueError(f"{who}: {name} has codes of shape {tuple(shape)}, not [rows, {width}] (K = {K} padded to {Kp})")
+    rows = shape[0]
+    if s.shape != (Kp // 128, rows, 4):
+        raise ValueError(f"{who}: {name} has scales of shape {tuple(s.shape)}, not {(Kp // 128, rows, 4)}")
+    cp, sp = c.data_ptr(), s.data_ptr()
+    ldc, one = c.stride()
+    ss, row, byte = s.stride()
+    if rows <= 1:
+        ldc, row = width, 4
+    if rows and (one != 1 or ldc < width or ldc % 16 or cp % 16):
+        raise ValueError(f"{who}: {name} has code rows that are not contiguous, or not 16-byte aligned")
+    if rows and (byte != 1 or row != 4 or ss < 4 * rows or ss % 4 or sp % 4):
+        raise ValueError(f"{who}: {name} has scales whose rows of a group are not 4 bytes apart")
+    return rows, ldc, ss, cp, sp
 
 
-def _mat(t, who, name, cols=None, rows=None):
+def _mat(t, who, name, rows=None, cols=None):
     """Row pitch in elements of a [rows, cols] matrix with contiguous rows."""
-    _need(t.dim() == 2, f"{who}: {name} has {t.dim()} dimensions, not 2")
-    _need(t.dtype in _DT3, f"{who}: {name} is {t.dtype}, not float16, bfloat16 or float32")
-    _need(max(t.shape) < 1 << 31, f"{who}: {name} has {max(t.shape)} rows or columns")
-    _need((rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols),
-          f"{who}: {name} has shape {tuple(t.shape)}, not {(t.shape[0] if rows is None else rows, t.shape[1] if cols is None else cols)}")
-    _need(t.numel() == 0 or t.shape[1] == 1 or t.stride(1) == 1, f"{who}: rows of {name} are not contiguous")
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    _need(t.numel() == 0 or ld >= t.shape[1], f"{who}: rows of {name} overlap")
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{who}: {name} has {len(shape)} dimensions, not 2")
+    if t.dtype not in _DT3:
+        raise ValueError(f"{who}: {name} is {t.dtype}, not float16, bfloat16 or float32")
+    m, n = shape
+    if (rows is not None and m != rows) or (cols is not None and n != cols) or m > _INT_MAX or n > _INT_MAX:
+        raise ValueError(f"{who}: {name} has shape {(m, n)}, not {(m if rows is None else rows, n if cols is None else cols)} (each under 2^31)")
+    ld, one = t.stride()
+    if m <= 1:
+        ld = n
+    if m and n > 1 and one != 1:
+        raise ValueError(f"{who}: rows of {name} are not contiguous")
+    if m and ld < n:
+        raise ValueError(f"{who}: rows of {name} overlap")
     return ld
 
 
 def _vec_f32(t, who, name, n):
-    _need(t.dtype == torch.float32 and tuple(t.shape) == (n,) and t.is_contiguous(), f"{who}: {name} has to be a contiguous float32 [{n}]")
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} has to be a contiguous float32 [{n}], is {t.dtype} {tuple(t.shape)}")
 
 
-def _call_on(who, tensors, name, *args):
-    """Calls an entry on the current stream of the device that all of the tensors are on."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise ValueError(f"{who}: tensors are on {dev}; there is no CPU form")
-    if dev.index == torch.cuda.current_device():
-        call(name, _stream(), *args)
+def _same_device(who, first, *rest):
+    """The index of the device that all of the tensors (None: not given) are on."""
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{who}: tensors on {first.device} and {t.device}")
+    if dev < 0:
+        raise ValueError(f"{who}: tensors are on {first.device}; there is no CPU form")
+    return dev
+
+
+# the handle without the Stream object around it: 0.1 us instead of 2.7
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _call_on(dev, name, *args):
+    """Calls an entry on the current stream of device ``dev``."""
+    if dev == torch.cuda.current_device():
+        call(name, _raw_stream(dev), *args)
     else:
         with torch.cuda.device(dev):
-            call(name, _stream(), *args)
+            call(name, _raw_stream(dev), *args)
 
 
 def mx_quantize(x, fmt="fp4"):
     """``x`` [M, K] (fp16, bfloat16 or fp32, contiguous rows) as an ``MxTensor``: per block of 32 columns the scale
     2^(floor(log2 amax) - emax), emax 2 ("fp4") or 8 ("fp8"), and every value over its scale rounded to nearest even, saturated at 6 or
     448.  A block with a NaN or an infinity reads back as NaN."""
-    _need(fmt in _MX, f"mx_quantize: format {fmt!r} is not 'fp4' or 'fp8'")
+    if fmt not in _MX:
+        raise ValueError(f"mx_quantize: format {fmt!r} is not 'fp4' or 'fp8'")
     ld = _mat(x, "mx_quantize", "x")
     M, K = x.shape
-    _need(K > 0, "mx_quantize: x has no columns")
-    q = _mx_empty(M, K, fmt, x.device)
-    _call_on("mx_quantize", (x,), "csam_mx_quantize", _ptr(x), ld, _DT3[x.dtype], _ptr(q.codes), q.codes.shape[1], _ptr(q.scales), 4 * M,
+    if K == 0:
+        raise ValueError("mx_quantize: x has no columns")
+    dev = _same_device("mx_quantize", x)
+    q = _mx_empty(x, M, K, fmt)
+    _call_on(dev, "csam_mx_quantize", x.data_ptr(), ld, _DT3[x.dtype], q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), 4 * M,
              _MX[fmt], M, K)
     return q
 
@@ -1280,12 +1304,12 @@ def mx_quantize(x, fmt="fp4"):
 def mx_dequantize(q, out_dtype=torch.float32):
     """The values [rows, K] an ``MxTensor`` stands for, rounded to ``out_dtype`` (exact in fp32; in bfloat16 too but for values below its
     smallest)."""
-    _need(out_dtype in _DT3, f"mx_dequantize: no output in {out_dtype}")
-    ldc, ss = _mx_check(q, "mx_dequantize", "q")
-    M = q.codes.shape[0]
-    y = torch.empty((M, q.K), dtype=out_dtype, device=q.codes.device)
-    _call_on("mx_dequantize", (q.codes, q.scales), "csam_mx_dequantize", _ptr(q.codes), ldc, _ptr(q.scales), ss, _MX[q.fmt], _ptr(y), q.K,
-             _DT3[out_dtype], M, q.K)
+    if out_dtype not in _DT3:
+        raise ValueError(f"mx_dequantize: no output in {out_dtype}")
+    M, ldc, ss, cp, sp = _mx_check(q, "mx_dequantize", "q")
+    dev = _same_device("mx_dequantize", q.codes, q.scales)
+    y = q.codes.new_empty((M, q.K), dtype=out_dtype)
+    _call_on(dev, "csam_mx_dequantize", cp, ldc, sp, ss, _MX[q.fmt], y.data_ptr(), q.K, _DT3[out_dtype], M, q.K)
     return y
 
 
@@ -1294,27 +1318,32 @@ def mx_gemm(a, w, out=None, bias=None, act=ACT_NONE, residual=None, out_dtype=to
     rounded once.  ``bias`` fp32 [N]; ``residual`` [M, N] fp16 / bfloat16 / fp32; ``out`` may be the residual.  The kernel and with it the
     order of the sum depend on the sizes: rows are not bitwise independent of M."""
     who = "mx_gemm"
-    _need(w.fmt == "fp4", f"{who}: w is in {w.fmt!r}; only 'fp4' weights are multiplied")
-    _need(a.K == w.K, f"{who}: a has K = {a.K}, w has K = {w.K}")
-    _need(a.K <= 1 << 20, f"{who}: K = {a.K} is over 2^20")
-    _need(act in (ACT_NONE, ACT_GELU, ACT_RELU), f"{who}: activation {act!r}")
-    lda, ass = _mx_check(a, who, "a")
-    ldw, wss = _mx_check(w, who, "w")
-    M, N = a.codes.shape[0], w.codes.shape[0]
-    ldr, r_dt = 0, 0
+    if w.fmt != "fp4":
+        raise ValueError(f"{who}: w is in {w.fmt!r}; only 'fp4' weights are multiplied")
+    K = a.K
+    if K != w.K or K > 1 << 20:
+        raise ValueError(f"{who}: a has K = {K}, w has K = {w.K} (equal, at most 2^20)")
+    if act not in (ACT_NONE, ACT_GELU, ACT_RELU):
+        raise ValueError(f"{who}: activation {act!r}")
+    M, lda, ass, ap, asp = _mx_check(a, who, "a")
+    N, ldw, wss, wp, wsp = _mx_check(w, who, "w")
+    ldr, r_dt, rp, bp = 0, 0, None, None
     if residual is not None:
-        ldr, r_dt = _mat(residual, who, "residual", N, M), _DT3[residual.dtype]
+        ldr, r_dt, rp = _mat(residual, who, "residual", M, N), _DT3[residual.dtype], residual.data_ptr()
     if bias is not None:
         _vec_f32(bias, who, "bias", N)
+        bp = bias.data_ptr()
     if out is None:
-        _need(out_dtype in _DT3, f"{who}: no output in {out_dtype}")
-        out = torch.empty((M, N), dtype=out_dtype, device=a.codes.device)
-        ldo = N
+        if out_dtype not in _DT3:
+            raise ValueError(f"{who}: no output in {out_dtype}")
+        dev, ldo = _same_device(who, a.codes, a.scales, w.codes, w.scales, bias, residual), N
+        out = a.codes.new_empty((M, N), dtype=out_dtype)
     else:
-        ldo = _mat(out, who, "out", N, M)
-    _call_on(who, (a.codes, a.scales, w.codes, w.scales, out, bias, residual), "csam_mx_gemm", _ptr(a.codes), lda, _ptr(a.scales), ass,
-             _MX[a.fmt], _ptr(w.codes), ldw, _ptr(w.scales), wss, _ptr(out), ldo, _DT3[out.dtype], _ptr(bias), _ptr(residual), ldr, r_dt,
-             act, M, N, a.K)
+        ldo = _mat(out, who, "out", M, N)
+        out_dtype = out.dtype
+        dev = _same_device(who, a.codes, a.scales, w.codes, w.scales, bias, residual, out)
+    _call_on(dev, "csam_mx_gemm", ap, lda, asp, ass, _MX[a.fmt], wp, ldw, wsp, wss, out.data_ptr(), ldo, _DT3[out_dtype], bp, rp, ldr, r_dt,
+             act, M, N, K)
     return out
 
 
@@ -1325,47 +1354,75 @@ def rms_norm(x, gamma, eps, residual=None, h_out=None, out_dtype=torch.float16):
     who = "rms_norm"
     ldx = _mat(x, who, "x")
     M, D = x.shape
-    _need(0 < D <= 32768, f"{who}: rows of {D} values (1 .. 32768)")
-    _need(eps > 0, f"{who}: eps has to be positive, got {eps}")
+    dt = x.dtype
+    if not 0 < D <= 32768:
+        raise ValueError(f"{who}: rows of {D} values (1 .. 32768)")
+    if not eps > 0:
+        raise ValueError(f"{who}: eps has to be positive, got {eps}")
     _vec_f32(gamma, who, "gamma", D)
-    _need(residual is not None or h_out is None, f"{who}: h_out without a residual")
-    ldr = ldh = r_dt = 0
+    mx = out_dtype in _MX
+    if not mx and out_dtype not in _DT3:
+        raise ValueError(f"{who}: no output in {out_dtype}")
+    ldr, ldh, r_dt, rp, hp = 0, 0, 0, None, None
     if residual is not None:
-        _need(residual.dtype in (x.dtype, torch.float32), f"{who}: the residual is {residual.dtype}; it has to be {x.dtype} or float32")
-        ldr, r_dt = _mat(residual, who, "residual", D, M), _DT3[residual.dtype]
+        rt = residual.dtype
+        if rt != dt and rt != torch.float32:
+            raise ValueError(f"{who}: the residual is {rt}; it has to be {dt} or float32")
+        ldr, r_dt, rp = _mat(residual, who, "residual", M, D), _DT3[rt], residual.data_ptr()
         if h_out is None:
-            h_out = torch.empty((M, D), dtype=residual.dtype, device=x.device)
-        _need(h_out.dtype == residual.dtype, f"{who}: h_out is {h_out.dtype}, the residual {residual.dtype}")
-        ldh = _mat(h_out, who, "h_out", D, M)
-    head = (_ptr(x), ldx, _DT3[x.dtype], _ptr(residual), ldr, r_dt, _ptr(h_out), ldh, _ptr(gamma), float(eps))
-    if out_dtype in _MX:
-        y = _mx_empty(M, D, out_dtype, x.device)
-        _call_on(who, (x, gamma, residual, h_out), "csam_rms_norm_mx", *head, _ptr(y.codes), y.codes.shape[1], _ptr(y.scales), 4 * M,
-                 _MX[out_dtype], M, D)
+            dev, ldh = _same_device(who, x, gamma, residual), D
+            h_out = residual.new_empty((M, D))
+        else:
+            if h_out.dtype != rt:
+                raise ValueError(f"{who}: h_out is {h_out.dtype}, the residual {rt}")
+            ldh = _mat(h_out, who, "h_out", M, D)
+            dev = _same_device(who, x, gamma, residual, h_out)
+        hp = h_out.data_ptr()
+    elif h_out is not None:
+        raise ValueError(f"{who}: h_out without a residual")
     else:
-        _need(out_dtype in _DT3, f"{who}: no output in {out_dtype}")
-        y = torch.empty((M, D), dtype=out_dtype, device=x.device)
-        _call_on(who, (x, gamma, residual, h_out), "csam_rms_norm", *head, _ptr(y), D, _DT3[out_dtype], M, D)
+        dev = _same_device(who, x, gamma)
+    if mx:
+        y = _mx_empty(x, M, D, out_dtype)
+        _call_on(dev, "csam_rms_norm_mx", x.data_ptr(), ldx, _DT3[dt], rp, ldr, r_dt, hp, ldh, gamma.data_ptr(), eps, y.codes.data_ptr(),
+                 y.codes.shape[1], y.scales.data_ptr(), 4 * M, _MX[out_dtype], M, D)
+    else:
+        y = x.new_empty((M, D), dtype=out_dtype)
+        _call_on(dev, "csam_rms_norm", x.data_ptr(), ldx, _DT3[dt], rp, ldr, r_dt, hp, ldh, gamma.data_ptr(), eps, y.data_ptr(), D,
+                 _DT3[out_dtype], M, D)
     return y if residual is None else (y, h_out)
 
 
 def rotary_frequencies(sections, theta=10000.0, device="cuda"):
     """(freq fp64 [pairs], axis int32 [pairs]) of ``rotary`` for ``sections[i]`` pairs of axis i, each axis with the geometric spectrum
     theta^(-j / sections[i])."""
-    _need(len(sections) > 0 and all(n > 0 for n in sections), f"rotary_frequencies: sections {sections}")
+    if not sections or min(sections) <= 0:
+        raise ValueError(f"rotary_frequencies: sections {sections}")
     freq = [float(theta) ** (-j / n) for n in sections for j in range(n)]
     axis = [i for i, n in enumerate(sections) for _ in range(n)]
     return torch.tensor(freq, dtype=torch.float64, device=device), torch.tensor(axis, dtype=torch.int32, device=device)
 
 
-def _heads(t, who, name, T, hd, written=False):
-    _need(t.dim() == 3 and t.shape[0] == T and t.shape[2] == hd and t.shape[1] > 0,
-          f"{who}: {name} has shape {tuple(t.shape)}, not [{T}, heads, {hd}]")
-    hs = t.stride(1) if t.shape[1] > 1 else hd
-    _need(T == 0 or ((hd == 1 or t.stride(2) == 1) and hd <= hs < 1 << 31), f"{who}: elements of a head of {name} are not contiguous, or heads overlap")
-    ld, H = (t.stride(0) if T > 1 else 0), t.shape[1]
-    _need(not written or T <= 1 or ld >= (H - 1) * hs + hd or (ld >= hd and hs >= (T - 1) * ld + hd), f"{who}: tokens of {name} overlap")
-    return ld, hs
+def _heads(t, who, name, T, hd, dtype, written=False):
+    """(heads, token pitch, head pitch) of [T, heads, hd] with contiguous heads."""
+    shape = t.shape
+    if t.dtype != dtype:
+        raise ValueError(f"{who}: {name} is {t.dtype}, q is {dtype}")
+    if len(shape) != 3 or shape[0] != T or shape[2] != hd or not 0 < shape[1] <= _INT_MAX:
+        raise ValueError(f"{who}: {name} has shape {tuple(shape)}, not [{T}, heads, {hd}]")
+    H = shape[1]
+    ld, hs, one = t.stride()
+    if H == 1:
+        hs = hd
+    if T == 0:
+        return H, 0, hd
+    if (hd > 1 and one != 1) or not hd <= hs <= _INT_MAX:
+        raise ValueError(f"{who}: elements of a head of {name} are not contiguous, or heads overlap")
+    if T == 1:
+        return H, 0, hs
+    if written and ld < (H - 1) * hs + hd and (ld < hd or hs < (T - 1) * ld + hd):
+        raise ValueError(f"{who}: tokens of {name} overlap")
+    return H, ld, hs
 
 
 def rotary(q, k, pos, freq, axis, interleaved=False, q_out=None, k_out=None):
@@ -1376,39 +1433,51 @@ def rotary(q, k, pos, freq, axis, interleaved=False, q_out=None, k_out=None):
     copied.  Returns (q_out, k_out), new tensors unless given; an output may be its input.  The gradient with respect to q and k is this
     call on the output's gradient with ``-pos``."""
     who = "rotary"
-    _need(q.dim() == 3, f"{who}: q has {q.dim()} dimensions, not 3")
-    T, Hq, hd = q.shape
-    _need(T < 1 << 31 and hd > 0, f"{who}: q has shape {tuple(q.shape)}")
-    _need(q.dtype in _DT3, f"{who}: q is {q.dtype}, not float16, bfloat16 or float32")
+    shape, dt = q.shape, q.dtype
+    if len(shape) != 3 or shape[0] > _INT_MAX or shape[2] == 0:
+        raise ValueError(f"{who}: q has shape {tuple(shape)}: {len(shape)} dimensions, not [tokens, heads, head_dim]")
+    if dt not in _DT3:
+        raise ValueError(f"{who}: q is {dt}, not float16, bfloat16 or float32")
+    T, _, hd = shape
     P = freq.numel()
-    _need(freq.dtype == torch.float64 and axis.dtype == torch.int32 and tuple(freq.shape) == tuple(axis.shape) == (P,)
-          and freq.is_contiguous() and axis.is_contiguous(), f"{who}: freq has to be float64 [pairs], axis int32 [pairs], both contiguous")
-    _need(0 < P and 2 * P <= hd, f"{who}: {P} pairs do not fit heads of {hd}")
-    _need(pos.dim() == 2 and pos.dtype in (torch.int32, torch.float32) and pos.shape[0] > 0, f"{who}: pos has to be int32 or float32 [axes, tokens]")
-    A, Tp = pos.shape
-    _need(T == 0 or (Tp > 0 and T % Tp == 0), f"{who}: {T} tokens are not a multiple of {Tp} positions")
-    _need(T == 0 or ((Tp == 1 or pos.stride(1) == 1) and (A == 1 or pos.stride(0) >= Tp)), f"{who}: positions of an axis are not contiguous")
+    if freq.dtype != torch.float64 or axis.dtype != torch.int32 or freq.shape != (P,) or axis.shape != (P,) or not (freq.is_contiguous() and axis.is_contiguous()):
+        raise ValueError(f"{who}: freq has to be float64 [pairs], axis int32 [pairs], both contiguous")
+    if not 0 < P <= hd // 2:
+        raise ValueError(f"{who}: {P} pairs do not fit heads of {hd}")
+    pt, ps = pos.dtype, pos.shape
+    if len(ps) != 2 or (pt != torch.int32 and pt != torch.float32) or not 0 < ps[0] <= _INT_MAX:
+        raise ValueError(f"{who}: pos has to be int32 or float32 [axes, tokens]")
+    A, Tp = ps
+    p_ld, p_one = pos.stride()
+    if A == 1:
+        p_ld = Tp
+    if T and (Tp == 0 or T % Tp):
+        raise ValueError(f"{who}: {T} tokens are not a multiple of {Tp} positions")
+    if T and ((Tp > 1 and p_one != 1) or p_ld < Tp):
+        raise ValueError(f"{who}: positions of an axis are not contiguous")
+    Hq, q_ld, q_hs = _heads(q, who, "q", T, hd, dt)
+    Hk = k_ld = k_hs = ko_ld = ko_hs = 0
+    kp = kop = None
+    if k is not None:
+        Hk, k_ld, k_hs = _heads(k, who, "k", T, hd, dt)
+    elif k_out is not None:
+        raise ValueError(f"{who}: k_out without k")
+    if q_out is not None:
+        Ho, qo_ld, qo_hs = _heads(q_out, who, "q_out", T, hd, dt, True)
+        if Ho != Hq:
+            raise ValueError(f"{who}: q_out has shape {tuple(q_out.shape)}, not {tuple(shape)}")
+    if k_out is not None:
+        Ho, ko_ld, ko_hs = _heads(k_out, who, "k_out", T, hd, dt, True)
+        if Ho != Hk:
+            raise ValueError(f"{who}: k_out has shape {tuple(k_out.shape)}, not {tuple(k.shape)}")
+    dev = _same_device(who, q, k, pos, freq, axis, q_out, k_out)
     if q_out is None:
-        q_out = torch.empty((T, Hq, hd), dtype=q.dtype, device=q.device)
-    outs = [(q, q_out, "q")]
+        q_out, qo_ld, qo_hs = q.new_empty((T, Hq, hd)), Hq * hd, hd
     if k is not None:
-        _heads(k, who, "k", T, hd)
         if k_out is None:
-            k_out = torch.empty((T, k.shape[1], hd), dtype=k.dtype, device=k.device)
-        outs.append((k, k_out, "k"))
-    else:
-        _need(k_out is None, f"{who}: k_out without k")
-    geo = []
-    for src, dst, name in outs:
-        _need(src.dtype == q.dtype and dst.dtype == q.dtype, f"{who}: {name} is {src.dtype} and {name}_out {dst.dtype}, q is {q.dtype}")
-        _need(src.shape == dst.shape, f"{who}: {name}_out has shape {tuple(dst.shape)}, not {tuple(src.shape)}")
-        geo.append((_heads(src, who, name, T, hd), _heads(dst, who, name + "_out", T, hd, True), src.shape[1]))
-    (q_ld, q_hs), (qo_ld, qo_hs), _ = geo[0]
-    if k is not None:
-        (k_ld, k_hs), (ko_ld, ko_hs), Hk = geo[1]
-    else:
-        k_ld = k_hs = ko_ld = ko_hs = Hk = 0
-    _call_on(who, (q, k, q_out, k_out, pos, freq, axis), "csam_rotary", _ptr(q), q_ld, q_hs, _ptr(q_out), qo_ld, qo_hs, Hq, _ptr(k), k_ld,
-             k_hs, _ptr(k_out), ko_ld, ko_hs, Hk, _DT3[q.dtype], _ptr(pos), max(pos.stride(0) if A > 1 else Tp, 1),
-             int(pos.dtype == torch.float32), _ptr(freq), _ptr(axis), A, P, int(bool(interleaved)), T, Tp, hd)
+            k_out, ko_ld, ko_hs = k.new_empty((T, Hk, hd)), Hk * hd, hd
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+    _call_on(dev, "csam_rotary", q.data_ptr(), q_ld, q_hs, q_out.data_ptr(), qo_ld, qo_hs, Hq, kp, k_ld, k_hs, kop, ko_ld, ko_hs, Hk, _DT3[dt],
+             pos.data_ptr(), p_ld or 1, 1 if pt == torch.float32 else 0, freq.data_ptr(), axis.data_ptr(), A, P, 1 if interleaved else 0, T,
+             Tp or 1, hd)
     return q_out, k_out

@@ -1,5 +1,8 @@
 """What the microscaled operators, the RMS norm and the rotary positions refuse, and the reference the GPU tests compare with.  The shape,
 type and stride checks come before anything touches a device, so they run here on CPU tensors."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -8,7 +11,7 @@ from crowdsam_amd import hip
 
 
 def mx(rows, K, fmt):
-    return hip._mx_empty(rows, K, fmt, "cpu")
+    return hip._mx_empty(torch.empty(0), rows, K, fmt)
 
 
 def test_reference_formats():
@@ -109,3 +112,19 @@ def test_entries_check_for_themselves():
     assert lib.csam_rms_norm(None, 64, 8, 0, 64, 8, 0, None, 8, 64, 1e-6, 64, 8, 0, 1, 8) == -1 and b"together" in lib.csam_last_error()
     assert lib.csam_rotary(None, 64, 8, 8, 64, 8, 8, 1, None, 0, 0, None, 0, 0, 0, 0, 64, 1, 0, 64, 64, 1, 5, 0, 1, 1, 8) == -1 and \
         b"pairs" in lib.csam_last_error()
+
+
+def test_gelu_polynomial_is_within_its_bound():
+    """The polynomial of Phi that 16-bit results take (csrc/csam_common.h), in float64 over the reals: |x P(x) - x Phi(x)| < 6.5e-5.  Beyond
+    the clamp both sides are within x (1 - Phi(x)) of each other, which only falls there."""
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "crowdsam_amd", "csrc", "csam_common.h")).read()
+    body = src[src.index("csam_gelu_poly2(float2_t x)"):]
+    c = float(re.search(r"const float c = ([0-9.]+)f;", body)[1])
+    k = [float(v) for v in re.search(r"k\[9\] = \{(.*?)\};", body, re.S)[1].replace("f", "").split(",")]
+    x = torch.linspace(-12, 12, 2_400_001, dtype=torch.float64)
+    xc = x.clamp(-c, c)
+    r = torch.full_like(x, k[0])
+    for v in k[1:]:
+        r = r * xc * xc + v
+    off = (x * (0.5 + xc * r) - x * 0.5 * torch.special.erfc(-x / 2 ** 0.5)).abs()
+    assert len(k) == 9 and float(off.max()) < 6.5e-5
