@@ -19,23 +19,24 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float csam_lo_bf16(unsigned u) { return __builtin_bit_cast(float, u << 16); }
 __device__ __forceinline__ float csam_hi_bf16(unsigned u) { return __builtin_bit_cast(float, u & 0xffff0000u); }
-template <typename T> __device__ __forceinline__ float csam_to_f32(T v) { return (float)v; }
 
-// 8 consecutive elements as fp32.  VEC: 16-byte aligned, all eight inside; otherwise `n` (<= 8, may be <= 0) of them, zeros behind.
+// N consecutive elements at an address that is a multiple of one element only: global accesses of any width take such addresses
+template <typename T, int N>
+struct csam_pack {
+  typedef T vec __attribute__((ext_vector_type(N)));
+  typedef vec at __attribute__((aligned(sizeof(T))));
+};
+// 8 consecutive elements as fp32; _tail: the first n of them (n may be <= 0), zeros behind
 template <typename T>
 __device__ __forceinline__ void csam_load8(const T* p, float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
-    const floatx4 a = *(const floatx4*)p, b = *(const floatx4*)(p + 4);
+    const auto a = *(const typename csam_pack<T, 4>::at*)p, b = *(const typename csam_pack<T, 4>::at*)(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-  } else if constexpr (__is_same(T, half_t)) {
-    const half8_t h = *(const half8_t*)p;
+  } else {
+    const auto h = *(const typename csam_pack<T, 8>::at*)p;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
-  } else {
-    const uintx4 u = *(const uintx4*)p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = csam_lo_bf16(u[i]), v[2 * i + 1] = csam_hi_bf16(u[i]);
   }
 }
 template <typename T>
@@ -47,14 +48,13 @@ __device__ __forceinline__ void csam_load8_tail(const T* p, int n, float (&v)[8]
 template <typename T>
 __device__ __forceinline__ void csam_store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
-    *(floatx4*)p = floatx4{v[0], v[1], v[2], v[3]};
-    *(floatx4*)(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
+    *(typename csam_pack<T, 4>::at*)p = floatx4{v[0], v[1], v[2], v[3]};
+    *(typename csam_pack<T, 4>::at*)(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
   } else {
-    typedef T vec8 __attribute__((ext_vector_type(8)));
-    vec8 h;
+    typename csam_pack<T, 8>::vec h;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = (T)v[i];
-    *(vec8*)p = h;
+    *(typename csam_pack<T, 8>::at*)p = h;
   }
 }
 template <typename T>

@@ -23,7 +23,7 @@ struct MxGemmArgs {
   const float* bias;
   const void* R; long ldr; int r_dt;
   int act, M, N, Kp;
-  int vec;                                   // 4 consecutive columns of C (and R, bias) may move as one access
+  int vec;                                   // N is a multiple of 4
 };
 
 typedef const __attribute__((address_space(1))) void* gptr_t;
@@ -48,38 +48,44 @@ __device__ __forceinline__ void mx_gelu4(floatx4& v, int c_dt) {
   }
 }
 
+// a NaN stays one
+__device__ __forceinline__ floatx4 mx_relu4(floatx4 v) {
+  return floatx4{v[0] < 0.f ? 0.f : v[0], v[1] < 0.f ? 0.f : v[1], v[2] < 0.f ? 0.f : v[2], v[3] < 0.f ? 0.f : v[3]};
+}
+
+// 4 elements at any element's address
+__device__ __forceinline__ floatx4 mx_load4(const void* p, int dt, long i) {
+  if (dt == CSAM_DT_F32) return *(const csam_pack<float, 4>::at*)((const float*)p + i);
+  if (dt == CSAM_DT_F16) {
+    const auto h = *(const csam_pack<half_t, 4>::at*)((const half_t*)p + i);
+    return floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+  }
+  const auto h = *(const csam_pack<bf16_t, 4>::at*)((const bf16_t*)p + i);
+  return floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+}
+__device__ __forceinline__ void mx_store4(void* p, int dt, long i, floatx4 v) {
+  if (dt == CSAM_DT_F32) *(csam_pack<float, 4>::at*)((float*)p + i) = v;
+  else if (dt == CSAM_DT_F16)
+    *(csam_pack<half_t, 4>::at*)((half_t*)p + i) = csam_pack<half_t, 4>::vec{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+  else *(csam_pack<bf16_t, 4>::at*)((bf16_t*)p + i) = csam_pack<bf16_t, 4>::vec{(bf16_t)v[0], (bf16_t)v[1], (bf16_t)v[2], (bf16_t)v[3]};
+}
+
 // 4 consecutive columns n .. n + 3 of row m: bias, activation, residual, rounding, store
 __device__ __forceinline__ void mx_epilogue4(const MxGemmArgs& p, int m, int n, floatx4 v) {
   if (m >= p.M || n >= p.N) return;
-  const bool full = p.vec && n + 4 <= p.N;
+  const bool full = n + 4 <= p.N;
   if (p.bias) {
-    if (full) v += *(const floatx4*)(p.bias + n);
+    if (full) v += mx_load4(p.bias, CSAM_DT_F32, n);
     else
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (n + i < p.N) v[i] += p.bias[n + i];
   }
   if (p.act == CSAM_ACT_GELU) mx_gelu4(v, p.c_dt);
-  else if (p.act == CSAM_ACT_RELU) v = floatx4{fmaxf(v[0], 0.f), fmaxf(v[1], 0.f), fmaxf(v[2], 0.f), fmaxf(v[3], 0.f)};
+  else if (p.act == CSAM_ACT_RELU) v = mx_relu4(v);
   if (full) {
-    if (p.R) {
-      const long at = (long)m * p.ldr + n;
-      if (p.r_dt == CSAM_DT_F32) v += *(const floatx4*)((const float*)p.R + at);
-      else if (p.r_dt == CSAM_DT_F16) {
-        const half4_t h = *(const half4_t*)((const half_t*)p.R + at);
-        v += floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-      } else {
-        const uintx2 u = *(const uintx2*)((const bf16_t*)p.R + at);
-        v += floatx4{csam_lo_bf16(u[0]), csam_hi_bf16(u[0]), csam_lo_bf16(u[1]), csam_hi_bf16(u[1])};
-      }
-    }
-    const long at = (long)m * p.ldc + n;
-    if (p.c_dt == CSAM_DT_F32) *(floatx4*)((float*)p.C + at) = v;
-    else if (p.c_dt == CSAM_DT_F16) *(half4_t*)((half_t*)p.C + at) = half4_t{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
-    else {
-      typedef bf16_t bf16x4_t __attribute__((ext_vector_type(4)));
-      *(bf16x4_t*)((bf16_t*)p.C + at) = bf16x4_t{(bf16_t)v[0], (bf16_t)v[1], (bf16_t)v[2], (bf16_t)v[3]};
-    }
+    if (p.R) v += mx_load4(p.R, p.r_dt, (long)m * p.ldr + n);
+    mx_store4(p.C, p.c_dt, (long)m * p.ldc + n, v);
     return;
   }
 #pragma unroll
@@ -98,7 +104,6 @@ __device__ __forceinline__ void mx_epilogue4(const MxGemmArgs& p, int m, int n, 
 // 4 consecutive columns of B rows STEP apart, all four inside N or none; every choice is uniform and made once for the B rows
 template <int B, int STEP>
 __device__ __forceinline__ void mx_epilogue_rows(const MxGemmArgs& p, int m, int n, floatx4 bz, floatx4 (&v)[B]) {
-  typedef bf16_t bf16x4_t __attribute__((ext_vector_type(4)));
   if (n >= p.N) return;
   floatx4 res[B];
   if (p.R) {
@@ -106,12 +111,13 @@ __device__ __forceinline__ void mx_epilogue_rows(const MxGemmArgs& p, int m, int
     if (p.r_dt == CSAM_DT_F32) {
 #pragma unroll
       for (int b = 0; b < B; ++b)
-        if (m + b * STEP < p.M) res[b] = *(const floatx4*)((const float*)p.R + at + (long)b * STEP * p.ldr);
+        if (m + b * STEP < p.M) res[b] = *(const csam_pack<float, 4>::at*)((const float*)p.R + at + (long)b * STEP * p.ldr);
     } else {
       uintx2 u[B];
 #pragma unroll
       for (int b = 0; b < B; ++b)
-        if (m + b * STEP < p.M) u[b] = *(const uintx2*)((const half_t*)p.R + at + (long)b * STEP * p.ldr);
+        if (m + b * STEP < p.M)
+          u[b] = __builtin_bit_cast(uintx2, *(const csam_pack<half_t, 4>::at*)((const half_t*)p.R + at + (long)b * STEP * p.ldr));
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         if (p.r_dt == CSAM_DT_F16) {
@@ -130,22 +136,16 @@ __device__ __forceinline__ void mx_epilogue_rows(const MxGemmArgs& p, int m, int
     for (int b = 0; b < B; ++b) mx_gelu4(v[b], p.c_dt);
   } else if (p.act == CSAM_ACT_RELU) {
 #pragma unroll
-    for (int b = 0; b < B; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[b][i] = v[b][i] > 0.f ? v[b][i] : 0.f;
+    for (int b = 0; b < B; ++b) v[b] = mx_relu4(v[b]);
   }
   if (p.R) {
 #pragma unroll
     for (int b = 0; b < B; ++b) v[b] += res[b];
   }
-  const long at = (long)m * p.ldc + n;
 #pragma unroll
   for (int b = 0; b < B; ++b) {
     if (m + b * STEP >= p.M) return;
-    const long o = at + (long)b * STEP * p.ldc;
-    if (p.c_dt == CSAM_DT_F32) *(floatx4*)((float*)p.C + o) = v[b];
-    else if (p.c_dt == CSAM_DT_F16) *(half4_t*)((half_t*)p.C + o) = half4_t{(half_t)v[b][0], (half_t)v[b][1], (half_t)v[b][2], (half_t)v[b][3]};
-    else *(bf16x4_t*)((bf16_t*)p.C + o) = bf16x4_t{(bf16_t)v[b][0], (bf16_t)v[b][1], (bf16_t)v[b][2], (bf16_t)v[b][3]};
+    mx_store4(p.C, p.c_dt, (long)(m + b * STEP) * p.ldc + n, v[b]);
   }
 }
 
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
   constexpr int LPR = COLS / 4, RPI = 64 / LPR, B = 4;     // lanes of a row, rows of an access, accesses of a batch
   float* buf = (float*)smem + wave * 32 * PITCH;
   const int n = bn0 + wn * COLS + (lane % LPR) * 4, mr = bm0 + wm * MI * 32 + lane / LPR;
-  const floatx4 bz = p.vec && p.bias && n < p.N ? *(const floatx4*)(p.bias + n) : floatx4{0.f, 0.f, 0.f, 0.f};
+  const floatx4 bz = p.vec && p.bias && n < p.N ? mx_load4(p.bias, CSAM_DT_F32, n) : floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -505,10 +505,7 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
   CSAM_REQUIRE(al(A_scales, a_scale_stride, 4) && al(W_scales, w_scale_stride, 4) && a_scale_stride >= 4L * M && w_scale_stride >= 4L * N,
                "csam_mx_gemm: scale groups have to lie 4-byte aligned, at least 4 * rows bytes apart");
   CSAM_REQUIRE(ldc >= N && (!residual || ldr >= N), "csam_mx_gemm: an output row pitch is shorter than N");
-  auto es = [](int dt) { return dt == CSAM_DT_F32 ? 4 : 2; };
-  const int vec = N % 4 == 0 && al(C, ldc * es(c_dtype), 4 * es(c_dtype)) && (!residual || al(residual, ldr * es(r_dtype), 4 * es(r_dtype))) &&
-                  (!bias || (uintptr_t)bias % 16 == 0);
   MxGemmArgs p = {(const uint8_t*)A, lda, (const uint8_t*)A_scales, a_scale_stride, (const uint8_t*)W, ldw, (const uint8_t*)W_scales,
-                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act, M, N, Kp, vec};
+                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act, M, N, Kp, N % 4 == 0};
   return a_fmt == CSAM_MX_FP8 ? mx_gemm_launch<CSAM_MX_FP8>((hipStream_t)stream, p) : mx_gemm_launch<CSAM_MX_FP4>((hipStream_t)stream, p);
 }

@@ -6,28 +6,29 @@
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------- quantise
-// A workgroup takes 32 rows x 256 columns: 512 bytes (16-bit inputs) of a row per half-wave, and a scale dword of 32 neighbouring
-// rows per 128 columns, i.e. a whole 128-byte line of scales per workgroup and group (no line is shared between XCDs).
-constexpr int Q_ROWS = 32, Q_COLS = 256;
+// A workgroup takes 8 R rows x 256 columns: 512 bytes (16-bit inputs) of a row per half-wave.  With R = 4 the scale dwords of its 32
+// neighbouring rows are a whole 128-byte line per 128 columns, and no line is shared between XCDs; R = 1 where that would leave CUs idle
+// (333 x 1001: 44 workgroups or 168, 5.3 or QR1 us).
+constexpr int Q_COLS = 256;
 
-template <typename T, int FMT>
+template <typename T, int FMT, int R>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, long ldx, uint8_t* __restrict__ codes, long ldc,
-                                                          uint8_t* __restrict__ scales, long sstride, int M, int K, int nseg, int vec) {
-  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * Q_ROWS + (threadIdx.x >> 5);
+                                                          uint8_t* __restrict__ scales, long sstride, int M, int K, int nseg) {
+  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * (8 * R) + (threadIdx.x >> 5);
   const int c8 = seg * (Q_COLS / 8) + (threadIdx.x & 31), k = c8 * 8;
-  float v[4][8];
+  float v[R][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int row = r0 + 8 * i;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
     if (row < M && k < K) {
-      if (vec && k + 8 <= K) csam_load8(x + (long)row * ldx + k, v[i]);
+      if (k + 8 <= K) csam_load8(x + (long)row * ldx + k, v[i]);
       else csam_load8_tail(x + (long)row * ldx + k, K - k, v[i]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int row = r0 + 8 * i;
     if (row < M) csam_mx_store8<FMT>(v[i], codes, ldc, scales, sstride, row, c8);       // whole half-waves share a row
   }
@@ -52,20 +53,20 @@ __device__ __forceinline__ void mx_values8(const uint8_t* codes, float scale, fl
   }
 }
 
-template <typename T, int FMT>
+template <typename T, int FMT, int R>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes, long ldc, const uint8_t* __restrict__ scales,
-                                                            long sstride, T* __restrict__ y, long ldy, int M, int K, int nseg, int vec) {
-  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * Q_ROWS + (threadIdx.x >> 5);
+                                                            long sstride, T* __restrict__ y, long ldy, int M, int K, int nseg) {
+  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * (8 * R) + (threadIdx.x >> 5);
   const int c8 = seg * (Q_COLS / 8) + (threadIdx.x & 31), k = c8 * 8;
   if (k >= K) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int row = r0 + 8 * i;
     if (row >= M) continue;
     const unsigned s = scales[(long)(c8 >> 4) * sstride + (long)row * 4 + ((c8 >> 2) & 3)];
     float v[8];
     mx_values8<FMT>(codes + row * ldc + (long)c8 * (FMT == CSAM_MX_FP4 ? 4 : 8), csam_e8m0(s), v);
-    if (vec && k + 8 <= K) csam_store8(y + (long)row * ldy + k, v);
+    if (k + 8 <= K) csam_store8(y + (long)row * ldy + k, v);
     else csam_store8_tail(y + (long)row * ldy + k, K - k, v);
   }
 }
@@ -82,7 +83,7 @@ struct RmsArgs {
   float eps;
   void* y; long ldy; int y_kind;          // CSAM_DT_*, or RMS_MX + CSAM_MX_*
   uint8_t* scales; long sstride;
-  int M, D, Dp, vec, gvec, rows;          // rows: rows of a row slot (a wave when NW = 1, the workgroup otherwise)
+  int M, D, Dp, rows;                     // rows: rows of a row slot (a wave when NW = 1, the workgroup otherwise)
 };
 constexpr int RMS_MX = 16;
 
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsAr
 #pragma unroll
   for (int j = 0; j < MAXC; ++j) {
     const int k = (c0 + j * STEP) * 8;
-    if (k + 8 <= D && p.gvec) csam_load8(p.gamma + k, g[j]);
+    if (k + 8 <= D) csam_load8(p.gamma + k, g[j]);
     else csam_load8_tail(p.gamma + k, D - k, g[j]);
   }
   const float inv_d = 1.0f / (float)D;
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsAr
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
       if (k < D) {
-        const bool full = p.vec && k + 8 <= D;
+        const bool full = k + 8 <= D;
         const T* xp = (const T*)p.x + row * p.ldx + k;
         if (full) csam_load8(xp, v[j]);
         else csam_load8_tail(xp, D - k, v[j]);
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsAr
           else csam_mx_store8<CSAM_MX_FP4>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
         }
       } else if (k < D) {
-        const bool full = p.vec && k + 8 <= D;
+        const bool full = k + 8 <= D;
         if (p.y_kind == CSAM_DT_F16) {
           half_t* yp = (half_t*)p.y + row * p.ldy + k;
           if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
@@ -220,12 +221,14 @@ int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* c
   CSAM_REQUIRE(dt_ok(x_dtype), "csam_mx_quantize: bad dtype %d", x_dtype);
   if (int rc = mx_check("csam_mx_quantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
   const int nseg = csam_cdiv(K, Q_COLS);
-  const long grid = (long)nseg * csam_cdiv(M, Q_ROWS);
+  const long grid = (long)nseg * csam_cdiv(M, 8);
   CSAM_REQUIRE(grid < (1L << 31), "csam_mx_quantize: too many elements");
-  const int vec = aligned(x, ldx * dt_bytes(x_dtype), 16);
   hipStream_t st = (hipStream_t)stream;
-#define GO(T, F) mx_quantize_kernel<T, F><<<(unsigned)grid, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, \
-                                                                         scale_stride, M, K, nseg, vec)
+#define GO(T, F)                                                                                                         \
+  do {                                                                                                                   \
+    if (grid >= 2048) mx_quantize_kernel<T, F, 4><<<(unsigned)((long)nseg * csam_cdiv(M, 32)), 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
+    else mx_quantize_kernel<T, F, 1><<<(unsigned)grid, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
+  } while (0)
   if (fmt == CSAM_MX_FP4) {
     if (x_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP4);
     else if (x_dtype == CSAM_DT_F32) GO(float, CSAM_MX_FP4);
@@ -248,12 +251,14 @@ int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void
   CSAM_REQUIRE(dt_ok(y_dtype), "csam_mx_dequantize: bad dtype %d", y_dtype);
   if (int rc = mx_check("csam_mx_dequantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
   const int nseg = csam_cdiv(K, Q_COLS);
-  const long grid = (long)nseg * csam_cdiv(M, Q_ROWS);
+  const long grid = (long)nseg * csam_cdiv(M, 8);
   CSAM_REQUIRE(grid < (1L << 31), "csam_mx_dequantize: too many elements");
-  const int vec = aligned(y, ldy * dt_bytes(y_dtype), 16);
   hipStream_t st = (hipStream_t)stream;
-#define GO(T, F) mx_dequantize_kernel<T, F><<<(unsigned)grid, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, \
-                                                                           scale_stride, (T*)y, ldy, M, K, nseg, vec)
+#define GO(T, F)                                                                                                         \
+  do {                                                                                                                   \
+    if (grid >= 2048) mx_dequantize_kernel<T, F, 4><<<(unsigned)((long)nseg * csam_cdiv(M, 32)), 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
+    else mx_dequantize_kernel<T, F, 1><<<(unsigned)grid, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
+  } while (0)
   if (fmt == CSAM_MX_FP4) {
     if (y_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP4);
     else if (y_dtype == CSAM_DT_F32) GO(float, CSAM_MX_FP4);
@@ -276,10 +281,6 @@ static int rms_any(hipStream_t st, RmsArgs& p, int x_dtype, int r_dtype, const c
   CSAM_REQUIRE(dt_ok(x_dtype), "%s: bad dtype %d", who, x_dtype);
   CSAM_REQUIRE(!p.r || r_dtype == x_dtype || r_dtype == CSAM_DT_F32, "%s: the residual is fp32 or of x's type", who);
   CSAM_REQUIRE(p.eps > 0.f, "%s: eps has to be positive", who);
-  p.vec = aligned(p.x, p.ldx * dt_bytes(x_dtype), 16) &&
-          (!p.r || (aligned(p.r, p.ldr * dt_bytes(r_dtype), 16) && aligned(p.h, p.ldh * dt_bytes(r_dtype), 16)));
-  if (p.y_kind < RMS_MX) p.vec = p.vec && aligned(p.y, p.ldy * dt_bytes(p.y_kind), 16);
-  p.gvec = (uintptr_t)p.gamma % 16 == 0;
   const int rk = !p.r ? 0 : (r_dtype == CSAM_DT_F32 && x_dtype != CSAM_DT_F32) ? 2 : 1;
 #define GO(T) return rk == 0 ? rms_launch<T, 0>(st, p) : rk == 1 ? rms_launch<T, 1>(st, p) : rms_launch<T, 2>(st, p)
   if (x_dtype == CSAM_DT_F16) GO(half_t);
@@ -292,7 +293,7 @@ int csam_rms_norm(void* stream, const void* x, long ldx, int x_dtype, const void
                   const float* gamma, float eps, void* y, long ldy, int y_dtype, int M, int D) {
   if (M == 0) return CSAM_OK;
   CSAM_REQUIRE(dt_ok(y_dtype) && ldy >= D, "csam_rms_norm: bad output dtype %d or row pitch %ld", y_dtype, ldy);
-  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0, 0, 0, 1};
+  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0, 1};
   return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm");
 }
 
@@ -302,7 +303,7 @@ int csam_rms_norm_mx(void* stream, const void* x, long ldx, int x_dtype, const v
   CSAM_REQUIRE(D > 0, "csam_rms_norm_mx: bad width %d", D);
   if (int rc = mx_check("csam_rms_norm_mx", codes, ldcodes, scales, scale_stride, fmt, M, D)) return rc;
   RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, codes, ldcodes, RMS_MX + fmt, (uint8_t*)scales, scale_stride, M, D,
-               csam_cdiv(D, 256) * 256, 0, 0, 1};
+               csam_cdiv(D, 256) * 256, 1};
   return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm_mx");
 }
 

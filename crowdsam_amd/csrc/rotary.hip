@@ -22,19 +22,19 @@ __device__ __forceinline__ void rotary_angle(const RotaryArgs& p, int t, int pai
   const double x = p.pos_f32 ? (double)((const float*)p.pos)[at] : (double)((const int*)p.pos)[at];
   const double turns = x * p.freq[pair] * 0.15915494309189533577;
   const float f = 2.0f * (float)(turns - __builtin_rint(turns));
-  c = cospif(f);
-  s = sinpif(f);
+  sincospif(f, &s, &c);
 }
 
-// One thread = one unit of one token for every `split`-th head: the angles are computed once and used for all of its heads.
-//   VEC, half:        VW elements of the first half of the pairs and their VW partners, or VW elements that pass through;
-//   VEC, interleaved: VW consecutive elements = VW / 2 pairs;
-//   scalar:           one pair, or one element that passes through.
+// One thread = one unit of one token for every `split`-th head: the angles are computed once and used for all of its heads, HB of which are
+// fetched together (the first HB before the angles are computed).
+//   half:        VW elements of the first half of the pairs and their VW partners, or VW elements that pass through;
+//   interleaved: VW consecutive elements = VW / 2 pairs.
 // Consecutive threads hold consecutive units of a head, then the next head phase: a wave touches whole runs of the row.
-template <typename T, bool HALF, bool VEC>
+template <typename T, bool HALF, int VW>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
-  constexpr int VW = VEC ? 16 / sizeof(T) : 1;
-  typedef T vec_t __attribute__((ext_vector_type(VW)));
+  typedef typename csam_pack<T, VW>::vec vec_t;
+  typedef typename csam_pack<T, VW>::at vec_at;
+  constexpr int HB = 4;
   const unsigned idx = blockIdx.x * 256u + threadIdx.x;
   const unsigned tw = idx / p.units;
   const int u = idx - tw * p.units;
@@ -44,81 +44,94 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
   const int H = p.Hq + p.Hk;
 
   // where the unit's elements are and what happens to them
-  int i0, i1 = -1;                                   // i1 < 0: only VW elements at i0
-  constexpr int NP = VEC ? (HALF ? VW : VW / 2) : 1;
+  constexpr int NP = HALF ? VW : VW / 2;
+  const int pair0 = u * NP;
+  const bool turn = pair0 < p.P;
+  const int i0 = HALF && !turn ? u * VW + p.P : u * VW;
+  vec_t v[HB], w[HB];
+  const bool lone = !HALF && VW == 2 && i0 + 1 == p.hd;        // the last element of a head of odd width
+  auto head = [&](int h, bool out) {
+    if (h < p.Hq) {
+      return out ? (char*)p.qo + ((long)t * p.ldqo + (long)h * p.hsqo) * (long)sizeof(T) : (char*)p.q + ((long)t * p.ldq + (long)h * p.hsq) * (long)sizeof(T);
+    }
+    h -= p.Hq;
+    return out ? (char*)p.ko + ((long)t * p.ldko + (long)h * p.hsko) * (long)sizeof(T) : (char*)p.k + ((long)t * p.ldk + (long)h * p.hsk) * (long)sizeof(T);
+  };
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+      const int h = h0 + b * p.split;
+      if (h < H) {
+        const T* src = (const T*)head(h, false);
+        if (!HALF && VW == 2 && lone) v[b][0] = src[i0];
+        else v[b] = *(const vec_at*)(src + i0);
+        if (HALF && turn) w[b] = *(const vec_at*)(src + i0 + p.P);
+      }
+    }
+  };
+  fetch(s0);
   float cs[NP], sn[NP];
-  bool turn = true;
-  if constexpr (VEC && HALF) {
-    turn = u * VW < p.P;
-    i0 = turn ? u * VW : u * VW + p.P;
-    if (turn) i1 = i0 + p.P;
-  } else if constexpr (VEC) {
-    i0 = u * VW;
-    turn = i0 < 2 * p.P;
-  } else {
-    turn = u < p.P;
-    i0 = turn ? (HALF ? u : 2 * u) : u + p.P;
-    if (turn) i1 = i0 + (HALF ? p.P : 1);
-  }
-  const int pair0 = VEC && !HALF ? u * NP : u * (VEC ? VW : 1);
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     cs[i] = 1.f, sn[i] = 0.f;
-    if (turn && pair0 + i < p.P) rotary_angle(p, (int)t, pair0 + i, cs[i], sn[i]);
+    if (pair0 + i < p.P) rotary_angle(p, (int)t, pair0 + i, cs[i], sn[i]);
   }
-  for (int h = s0; h < H; h += p.split) {
-    const bool isq = h < p.Hq;
-    const T* src = isq ? (const T*)p.q + (long)t * p.ldq + (long)h * p.hsq : (const T*)p.k + (long)t * p.ldk + (long)(h - p.Hq) * p.hsk;
-    T* dst = isq ? (T*)p.qo + (long)t * p.ldqo + (long)h * p.hsqo : (T*)p.ko + (long)t * p.ldko + (long)(h - p.Hq) * p.hsko;
-    if constexpr (VEC && !HALF) {
-      vec_t v = *(const vec_t*)(src + i0);
+  for (int h0 = s0; h0 < H; h0 += HB * p.split) {
+    if (h0 != s0) fetch(h0);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (pair0 + i < p.P) {                       // a pair behind the last one passes through bit for bit
-          const float a = (float)v[2 * i], b = (float)v[2 * i + 1];
-          v[2 * i] = (T)(a * cs[i] - b * sn[i]);
-          v[2 * i + 1] = (T)(a * sn[i] + b * cs[i]);
+    for (int b = 0; b < HB; ++b) {
+      const int h = h0 + b * p.split;
+      if (h >= H) break;
+      T* dst = (T*)head(h, true);
+      if constexpr (HALF) {
+        if (turn) {
+#pragma unroll
+          for (int i = 0; i < VW; ++i) {
+            const float x = (float)v[b][i], y = (float)w[b][i];
+            v[b][i] = (T)(x * cs[i] - y * sn[i]);
+            w[b][i] = (T)(x * sn[i] + y * cs[i]);
+          }
+          *(vec_at*)(dst + i0 + p.P) = w[b];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          if (pair0 + i < p.P) {                     // a pair behind the last one passes through bit for bit
+            const float x = (float)v[b][2 * i], y = (float)v[b][2 * i + 1];
+            v[b][2 * i] = (T)(x * cs[i] - y * sn[i]);
+            v[b][2 * i + 1] = (T)(x * sn[i] + y * cs[i]);
+          }
         }
       }
-      *(vec_t*)(dst + i0) = v;
-    } else {
-      vec_t v = *(const vec_t*)(src + i0);
-      if (i1 >= 0) {
-        vec_t w = *(const vec_t*)(src + i1);
-#pragma unroll
-        for (int i = 0; i < VW; ++i) {
-          const float a = (float)v[i], b = (float)w[i];
-          v[i] = (T)(a * cs[i] - b * sn[i]);
-          w[i] = (T)(a * sn[i] + b * cs[i]);
-        }
-        *(vec_t*)(dst + i1) = w;
-      }
-      *(vec_t*)(dst + i0) = v;
+      if (!HALF && VW == 2 && lone) dst[i0] = v[b][0];
+      else *(vec_at*)(dst + i0) = v[b];
     }
   }
 }
 
-template <typename T>
-int rotary_launch(hipStream_t st, RotaryArgs& p, int half) {
-  constexpr int VW = 16 / sizeof(T);
-  auto al = [&](const void* b, long ld, long hs) { return !b || ((uintptr_t)b % 16 == 0 && ld % VW == 0 && hs % VW == 0); };
-  const bool vec = al(p.q, p.ldq, p.hsq) && al(p.qo, p.ldqo, p.hsqo) && al(p.k, p.ldk, p.hsk) && al(p.ko, p.ldko, p.hsko) &&
-                   p.hd % VW == 0 && (!half || p.P % VW == 0);
-  p.units = !vec ? p.P + (p.hd - 2 * p.P) : half ? (p.hd - p.P) / VW : p.hd / VW;
+template <typename T, bool HALF, int VW>
+int rotary_go(hipStream_t st, RotaryArgs& p) {
+  p.units = csam_cdiv(HALF ? p.hd - p.P : p.hd, VW);
+  // heads of a thread: the angles cost a thread about as much as eight heads, but a small call wants threads more than it minds angles
   const int H = p.Hq + p.Hk;
-  p.split = csam_cdiv(H, 4);
-  const long n = (long)p.T * p.units * p.split;
+  const long per_head = (long)p.T * p.units;
+  p.split = per_head * csam_cdiv(H, 8) >= 262144 ? csam_cdiv(H, 8) : per_head * csam_cdiv(H, 4) >= 65536 ? csam_cdiv(H, 4) : H;
+  const long n = per_head * p.split;
   CSAM_REQUIRE(n < (1L << 31), "csam_rotary: too many elements");
-  const unsigned grid = (unsigned)csam_cdiv(n, 256);
-  if (vec) {
-    if (half) rotary_kernel<T, true, true><<<grid, 256, 0, st>>>(p);
-    else rotary_kernel<T, false, true><<<grid, 256, 0, st>>>(p);
-  } else {
-    if (half) rotary_kernel<T, true, false><<<grid, 256, 0, st>>>(p);
-    else rotary_kernel<T, false, false><<<grid, 256, 0, st>>>(p);
-  }
+  rotary_kernel<T, HALF, VW><<<(unsigned)csam_cdiv(n, 256), 256, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_rotary");
   return CSAM_OK;
+}
+
+// the widest accesses that units of whole accesses allow (addresses need no alignment beyond an element's)
+template <typename T>
+int rotary_launch(hipStream_t st, RotaryArgs& p, int half) {
+  constexpr int W = 16 / sizeof(T);
+  const int odd = half ? p.P | p.hd : p.hd;
+  if (odd % W == 0) return half ? rotary_go<T, true, W>(st, p) : rotary_go<T, false, W>(st, p);
+  if (W == 8 && odd % 4 == 0) return half ? rotary_go<T, true, 4>(st, p) : rotary_go<T, false, 4>(st, p);
+  if (!half) return rotary_go<T, false, 2>(st, p);
+  return odd % 2 == 0 ? rotary_go<T, true, 2>(st, p) : rotary_go<T, true, 1>(st, p);
 }
 
 }  // namespace
