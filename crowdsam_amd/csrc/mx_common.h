@@ -26,6 +26,12 @@ struct csam_pack {
   typedef T vec __attribute__((ext_vector_type(N)));
   typedef vec at __attribute__((aligned(sizeof(T))));
 };
+// store; NT: past the caches' retention, for results that no cache would hold until they are read
+template <bool NT, typename P, typename V>
+__device__ __forceinline__ void csam_put(P* p, V v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
 // 8 consecutive elements as fp32; _tail: the first n of them (n may be <= 0), zeros behind
 template <typename T>
 __device__ __forceinline__ void csam_load8(const T* p, float (&v)[8]) {
@@ -45,16 +51,16 @@ __device__ __forceinline__ void csam_load8_tail(const T* p, int n, float (&v)[8]
   for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
 }
 // 8 consecutive elements, rounded to nearest even
-template <typename T>
+template <bool NT = false, typename T>
 __device__ __forceinline__ void csam_store8(T* p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
-    *(typename csam_pack<T, 4>::at*)p = floatx4{v[0], v[1], v[2], v[3]};
-    *(typename csam_pack<T, 4>::at*)(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
+    csam_put<NT>((typename csam_pack<T, 4>::at*)p, floatx4{v[0], v[1], v[2], v[3]});
+    csam_put<NT>((typename csam_pack<T, 4>::at*)(p + 4), floatx4{v[4], v[5], v[6], v[7]});
   } else {
     typename csam_pack<T, 8>::vec h;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = (T)v[i];
-    *(typename csam_pack<T, 8>::at*)p = h;
+    csam_put<NT>((typename csam_pack<T, 8>::at*)p, h);
   }
 }
 template <typename T>
@@ -121,14 +127,14 @@ __device__ __forceinline__ unsigned csam_mx_quant8(const float (&v)[8], unsigned
 
 // Codes and scales of chunk `c8` (8 elements) of row `row`; 16 consecutive lanes hold a 128-wide group, so the four block bytes are
 // put together with two rotations within 16 lanes and leave as one dword.
-template <int FMT>
+template <int FMT, bool NT = false>
 __device__ __forceinline__ void csam_mx_store8(const float (&v)[8], uint8_t* codes, long ldc, uint8_t* scales, long sstride, long row,
                                                int c8) {
   unsigned c[2];
   unsigned s = csam_mx_quant8<FMT>(v, c) << (8 * ((c8 >> 2) & 3));
   s |= csam_dpp<0x124>(s);                                // row_ror:4
   s |= csam_dpp<0x128>(s);                                // row_ror:8
-  if constexpr (FMT == CSAM_MX_FP4) *(unsigned*)(codes + row * ldc + c8 * 4) = c[0];
-  else *(uintx2*)(codes + row * ldc + c8 * 8) = uintx2{c[0], c[1]};
+  if constexpr (FMT == CSAM_MX_FP4) csam_put<NT>((unsigned*)(codes + row * ldc + c8 * 4), c[0]);
+  else csam_put<NT>((uintx2*)(codes + row * ldc + c8 * 8), uintx2{c[0], c[1]});
   if ((c8 & 15) == 0) *(unsigned*)(scales + (long)(c8 >> 4) * sstride + row * 4) = s;
 }

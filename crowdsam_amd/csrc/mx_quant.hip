@@ -8,10 +8,11 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------- quantise
 // A workgroup takes 8 R rows x 256 columns: 512 bytes (16-bit inputs) of a row per half-wave.  With R = 4 the scale dwords of its 32
 // neighbouring rows are a whole 128-byte line per 128 columns, and no line is shared between XCDs; R = 1 where that would leave CUs idle
-// (333 x 1001: 44 workgroups or 168, 5.3 or QR1 us).
+// (333 x 1001: 44 workgroups or 168, 5.3 or 2.5 us).  NT: codes that the L2s would not
+// hold are stored past them (21320 x 4096 fp16 to E4M3: 52.4 us, 47.5 so).
 constexpr int Q_COLS = 256;
 
-template <typename T, int FMT, int R>
+template <typename T, int FMT, int R, bool NT>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, long ldx, uint8_t* __restrict__ codes, long ldc,
                                                           uint8_t* __restrict__ scales, long sstride, int M, int K, int nseg) {
   const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * (8 * R) + (threadIdx.x >> 5);
@@ -30,7 +31,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = r0 + 8 * i;
-    if (row < M) csam_mx_store8<FMT>(v[i], codes, ldc, scales, sstride, row, c8);       // whole half-waves share a row
+    if (row < M) csam_mx_store8<FMT, NT>(v[i], codes, ldc, scales, sstride, row, c8);       // whole half-waves share a row
   }
 }
 
@@ -226,8 +227,10 @@ int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* c
   hipStream_t st = (hipStream_t)stream;
 #define GO(T, F)                                                                                                         \
   do {                                                                                                                   \
-    if (grid >= 2048) mx_quantize_kernel<T, F, 4><<<(unsigned)((long)nseg * csam_cdiv(M, 32)), 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
-    else mx_quantize_kernel<T, F, 1><<<(unsigned)grid, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
+    const unsigned g4 = (unsigned)((long)nseg * csam_cdiv(M, 32));                                                       \
+    if ((long)M * ldcodes > (32L << 20)) mx_quantize_kernel<T, F, 4, true><<<g4, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
+    else if (grid >= 2048) mx_quantize_kernel<T, F, 4, false><<<g4, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
+    else mx_quantize_kernel<T, F, 1, false><<<(unsigned)grid, 256, 0, st>>>((const T*)x, ldx, (uint8_t*)codes, ldcodes, (uint8_t*)scales, scale_stride, M, K, nseg); \
   } while (0)
   if (fmt == CSAM_MX_FP4) {
     if (x_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP4);

@@ -11,114 +11,138 @@ struct RotaryArgs {
   const void* pos; long pos_stride; int pos_f32;    // [axes][Tp]
   const double* freq; const int* axis;              // [P] radians per unit, axis of each pair
   int T, Tp, Hq, Hk, hd, P, axes;
-  int units, split;                                 // units of a head, head phases of a token
+  int tokens, heads, splits;                        // tokens and heads of a workgroup, workgroups that share a token's heads
+  int units, Pp;                                    // units of a head; P rounded up to whole 16-byte table reads
+  unsigned by_unit, by_token, by_pair;              // ceil(2^32 / d) for d = units, heads * units, P
 };
+constexpr int ROT_TABLE = 2048;                     // (cos, sin) entries of a workgroup's table: 16 KB
+
+// n / d by d's reciprocal: exact while n * d < 2^32, and every n here is below 2^16
+__device__ __forceinline__ unsigned rot_div(unsigned n, unsigned r, int d) { return d == 1 ? n : __umulhi(n, r); }
 
 // cos and sin of pos * freq.  The product and its reduction to one turn are in fp64: at a position of 1e5 an fp32 angle is off by
 // 4e-3 radians.  What is left is in [-1/2, 1/2] turns, where the fp32 functions are exact to an ulp.
-__device__ __forceinline__ void rotary_angle(const RotaryArgs& p, int t, int pair, float& c, float& s) {
+__device__ __forceinline__ float2_t rotary_angle(const RotaryArgs& p, int t, int pair) {
+  // a token's positions do not depend on the pair's axis: those of the first four axes are fetched beside it
+  const int at = t % p.Tp;
+  int w[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) w[a] = a < p.axes ? ((const int*)p.pos)[(long)a * p.pos_stride + at] : 0;
+  const double f = p.freq[pair];
   const int ax = min(max(p.axis[pair], 0), p.axes - 1);
-  const long at = (long)ax * p.pos_stride + t % p.Tp;
-  const double x = p.pos_f32 ? (double)((const float*)p.pos)[at] : (double)((const int*)p.pos)[at];
-  const double turns = x * p.freq[pair] * 0.15915494309189533577;
-  const float f = 2.0f * (float)(turns - __builtin_rint(turns));
-  sincospif(f, &s, &c);
+  int v = ax == 0 ? w[0] : ax == 1 ? w[1] : ax == 2 ? w[2] : w[3];
+  if (ax > 3) v = ((const int*)p.pos)[(long)ax * p.pos_stride + at];
+  const double x = p.pos_f32 ? (double)__builtin_bit_cast(float, v) : (double)v;
+  const double turns = x * f * 0.15915494309189533577;
+  float c, s;
+  sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &s, &c);
+  return float2_t{c, s};
 }
 
-// One thread = one unit of one token for every `split`-th head: the angles are computed once and used for all of its heads, HB of which are
-// fetched together (the first HB before the angles are computed).
+// A workgroup takes `tokens` tokens x `heads` heads: it puts cos and sin of each of its tokens and pairs into LDS once, and walks its
+// units, HB of a thread's at a time, the first of them fetched before the angles are computed:
 //   half:        VW elements of the first half of the pairs and their VW partners, or VW elements that pass through;
 //   interleaved: VW consecutive elements = VW / 2 pairs.
-// Consecutive threads hold consecutive units of a head, then the next head phase: a wave touches whole runs of the row.
-template <typename T, bool HALF, int VW>
+// Consecutive threads hold consecutive units of a head, then the next head: a wave touches whole runs of the row.
+template <typename T, bool HALF, int VW, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
   typedef typename csam_pack<T, VW>::vec vec_t;
   typedef typename csam_pack<T, VW>::at vec_at;
-  constexpr int HB = 4;
-  const unsigned idx = blockIdx.x * 256u + threadIdx.x;
-  const unsigned tw = idx / p.units;
-  const int u = idx - tw * p.units;
-  const unsigned t = tw / p.split;
-  const int s0 = tw - t * p.split;
-  if (t >= (unsigned)p.T) return;
-  const int H = p.Hq + p.Hk;
+  constexpr int HB = 4, NP = HALF ? VW : VW / 2;
+  __shared__ __attribute__((aligned(16))) float2_t table[ROT_TABLE];
+  const int hb = blockIdx.x % p.splits * p.heads;
+  const int t0 = (int)(blockIdx.x / p.splits) * p.tokens, nt = min(p.tokens, p.T - t0);
+  const int H = p.Hq + p.Hk, per_token = p.heads * p.units, total = nt * per_token;
 
-  // where the unit's elements are and what happens to them
-  constexpr int NP = HALF ? VW : VW / 2;
-  const int pair0 = u * NP;
-  const bool turn = pair0 < p.P;
-  const int i0 = HALF && !turn ? u * VW + p.P : u * VW;
   vec_t v[HB], w[HB];
-  const bool lone = !HALF && VW == 2 && i0 + 1 == p.hd;        // the last element of a head of odd width
-  auto head = [&](int h, bool out) {
-    if (h < p.Hq) {
-      return out ? (char*)p.qo + ((long)t * p.ldqo + (long)h * p.hsqo) * (long)sizeof(T) : (char*)p.q + ((long)t * p.ldq + (long)h * p.hsq) * (long)sizeof(T);
-    }
-    h -= p.Hq;
-    return out ? (char*)p.ko + ((long)t * p.ldko + (long)h * p.hsko) * (long)sizeof(T) : (char*)p.k + ((long)t * p.ldk + (long)h * p.hsk) * (long)sizeof(T);
-  };
-  auto fetch = [&](int h0) {
+  T* dst[HB];                                       // where the unit goes; null: no unit
+  short pair0[HB], tl[HB];
+  auto fetch = [&](int first) {
 #pragma unroll
     for (int b = 0; b < HB; ++b) {
-      const int h = h0 + b * p.split;
-      if (h < H) {
-        const T* src = (const T*)head(h, false);
-        if (!HALF && VW == 2 && lone) v[b][0] = src[i0];
-        else v[b] = *(const vec_at*)(src + i0);
-        if (HALF && turn) w[b] = *(const vec_at*)(src + i0 + p.P);
-      }
+      const int idx = first + b * 256;
+      dst[b] = nullptr;
+      if (idx >= total) continue;
+      const int tk = (int)rot_div(idx, p.by_token, per_token), r = idx - tk * per_token, hl = (int)rot_div(r, p.by_unit, p.units), u = r - hl * p.units;
+      const int h = hb + hl;
+      if (h >= H) continue;
+      const long t = t0 + tk;
+      pair0[b] = (short)(u * NP);
+      tl[b] = (short)tk;
+      const int i0 = HALF && u * NP >= p.P ? u * VW + p.P : u * VW;
+      const bool isq = h < p.Hq;
+      const T* src = (isq ? (const T*)p.q + t * p.ldq + (long)h * p.hsq : (const T*)p.k + t * p.ldk + (long)(h - p.Hq) * p.hsk) + i0;
+      dst[b] = (isq ? (T*)p.qo + t * p.ldqo + (long)h * p.hsqo : (T*)p.ko + t * p.ldko + (long)(h - p.Hq) * p.hsko) + i0;
+      if (!HALF && VW == 2 && i0 + 1 == p.hd) v[b][0] = src[0];            // the last element of a head of odd width
+      else v[b] = *(const vec_at*)src;
+      if (HALF && u * NP < p.P) w[b] = *(const vec_at*)(src + p.P);
     }
   };
-  fetch(s0);
-  float cs[NP], sn[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    cs[i] = 1.f, sn[i] = 0.f;
-    if (pair0 + i < p.P) rotary_angle(p, (int)t, pair0 + i, cs[i], sn[i]);
+  fetch(threadIdx.x);
+  for (int i = threadIdx.x; i < nt * p.P; i += 256) {
+    const int tk = (int)rot_div(i, p.by_pair, p.P), pair = i - tk * p.P;
+    table[tk * p.Pp + pair] = rotary_angle(p, t0 + tk, pair);
   }
-  for (int h0 = s0; h0 < H; h0 += HB * p.split) {
-    if (h0 != s0) fetch(h0);
+  __syncthreads();
+  for (int first = threadIdx.x; first < total; first += 256 * HB) {
+    if (first != (int)threadIdx.x) fetch(first);
 #pragma unroll
     for (int b = 0; b < HB; ++b) {
-      const int h = h0 + b * p.split;
-      if (h >= H) break;
-      T* dst = (T*)head(h, true);
+      if (!dst[b]) continue;
+      const bool turn = pair0[b] < p.P;
+      float2_t cs[NP];
+      if (turn) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) cs[i] = table[tl[b] * p.Pp + pair0[b] + i];
+      }
       if constexpr (HALF) {
         if (turn) {
 #pragma unroll
           for (int i = 0; i < VW; ++i) {
             const float x = (float)v[b][i], y = (float)w[b][i];
-            v[b][i] = (T)(x * cs[i] - y * sn[i]);
-            w[b][i] = (T)(x * sn[i] + y * cs[i]);
+            v[b][i] = (T)(x * cs[i][0] - y * cs[i][1]);
+            w[b][i] = (T)(x * cs[i][1] + y * cs[i][0]);
           }
-          *(vec_at*)(dst + i0 + p.P) = w[b];
+          csam_put<NT>((vec_at*)(dst[b] + p.P), w[b]);
         }
+        csam_put<NT>((vec_at*)dst[b], v[b]);
       } else {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          if (pair0 + i < p.P) {                     // a pair behind the last one passes through bit for bit
+          if (pair0[b] + i < p.P) {                  // a pair behind the last one passes through bit for bit
             const float x = (float)v[b][2 * i], y = (float)v[b][2 * i + 1];
-            v[b][2 * i] = (T)(x * cs[i] - y * sn[i]);
-            v[b][2 * i + 1] = (T)(x * sn[i] + y * cs[i]);
+            v[b][2 * i] = (T)(x * cs[i][0] - y * cs[i][1]);
+            v[b][2 * i + 1] = (T)(x * cs[i][1] + y * cs[i][0]);
           }
         }
+        if (VW == 2 && pair0[b] * 2 + 1 == p.hd) dst[b][0] = v[b][0];
+        else csam_put<NT>((vec_at*)dst[b], v[b]);
       }
-      if (!HALF && VW == 2 && lone) dst[i0] = v[b][0];
-      else *(vec_at*)(dst + i0) = v[b];
     }
   }
 }
 
 template <typename T, bool HALF, int VW>
 int rotary_go(hipStream_t st, RotaryArgs& p) {
+  constexpr int NP = HALF ? VW : VW / 2, HB = 4;
   p.units = csam_cdiv(HALF ? p.hd - p.P : p.hd, VW);
-  // heads of a thread: the angles cost a thread about as much as eight heads, but a small call wants threads more than it minds angles
+  p.Pp = csam_cdiv(p.P, NP > 2 ? NP : 2) * (NP > 2 ? NP : 2);
   const int H = p.Hq + p.Hk;
-  const long per_head = (long)p.T * p.units;
-  p.split = per_head * csam_cdiv(H, 8) >= 262144 ? csam_cdiv(H, 8) : per_head * csam_cdiv(H, 4) >= 65536 ? csam_cdiv(H, 4) : H;
-  const long n = per_head * p.split;
-  CSAM_REQUIRE(n < (1L << 31), "csam_rotary: too many elements");
-  rotary_kernel<T, HALF, VW><<<(unsigned)csam_cdiv(n, 256), 256, 0, st>>>(p);
+  // A workgroup's units: one batch of its threads (16384 tokens x 32 heads of 80: 39.8 us, 45.4 with two batches).  A token with more is
+  // shared by workgroups, tokens with fewer share one; a call that would not give every CU a workgroup this way is cut finer.
+  const long all = (long)p.T * H * p.units, want = all >= 256L * 256 * HB ? 256 * HB : max(256L, all / 256);
+  p.heads = (int)max(1L, min((long)H, want / p.units));
+  p.splits = csam_cdiv(H, p.heads);
+  p.tokens = (int)max(1L, min(min((long)p.T, (long)ROT_TABLE / p.Pp), want / ((long)p.heads * p.units)));
+  auto recip = [](long d) { return (unsigned)(((1ULL << 32) + d - 1) / d); };
+  p.by_unit = recip(p.units);
+  p.by_token = recip((long)p.heads * p.units);
+  p.by_pair = recip(p.P);
+  const long grid = (long)csam_cdiv(p.T, p.tokens) * p.splits;
+  CSAM_REQUIRE(grid < (1L << 31), "csam_rotary: too many elements");
+  // results beyond the L2s' size are stored past them (the same call: 39.8 us, 33.0 so)
+  if (all * VW * (long)sizeof(T) > (32L << 20)) rotary_kernel<T, HALF, VW, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  else rotary_kernel<T, HALF, VW, false><<<(unsigned)grid, 256, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_rotary");
   return CSAM_OK;
 }
@@ -145,11 +169,12 @@ extern "C" int csam_rotary(void* stream, const void* q, long ldq, int hsq, void*
   CSAM_REQUIRE(T > 0 && Hq > 0 && Hk >= 0 && head_dim > 0 && axes > 0, "csam_rotary: bad sizes T %d Hq %d Hk %d head_dim %d axes %d", T, Hq, Hk,
                head_dim, axes);
   CSAM_REQUIRE(pairs > 0 && 2 * (long)pairs <= head_dim, "csam_rotary: %d pairs do not fit a head of %d", pairs, head_dim);
+  CSAM_REQUIRE(head_dim <= 2 * ROT_TABLE, "csam_rotary: heads of %d elements (at most %d)", head_dim, 2 * ROT_TABLE);
   CSAM_REQUIRE(T_pos > 0 && T % T_pos == 0 && pos_stride >= T_pos, "csam_rotary: %d tokens are not a multiple of %d positions", T, T_pos);
   CSAM_REQUIRE(dtype == CSAM_DT_F16 || dtype == CSAM_DT_F32 || dtype == CSAM_DT_BF16, "csam_rotary: bad dtype %d", dtype);
   CSAM_REQUIRE(hsq >= head_dim && hsqo >= head_dim && (!Hk || (hsk >= head_dim && hsko >= head_dim)), "csam_rotary: heads overlap");
   RotaryArgs p = {q, q_out, ldq, ldqo, Hk ? k : nullptr, Hk ? k_out : nullptr, ldk, ldko, hsq, hsqo, hsk, hsko, pos, pos_stride, pos_is_f32,
-                  freq, axis, T, T_pos, Hq, Hk, head_dim, pairs, axes, 0, 0};
+                  freq, axis, T, T_pos, Hq, Hk, head_dim, pairs, axes, 0, 0, 0, 0, 0, 0, 0, 0};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CSAM_DT_F16) return rotary_launch<half_t>(st, p, !interleaved);
   if (dtype == CSAM_DT_BF16) return rotary_launch<bf16_t>(st, p, !interleaved);
