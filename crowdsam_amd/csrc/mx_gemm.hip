@@ -456,13 +456,21 @@ int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
   return CSAM_OK;
 }
 
-// Which form: the largest tile that still fills the chip, since the products move their operands L2 -> LDS at 7 to 9 TB/s and are bound by
-// that before the matrix units; us on one MI355X (M x N x K, fp16 out, no epilogue), E2M1 / E4M3 activations:
-//   rows      against 64x64      32 x 4096 x 4096:    5.8 / 7.7    against  7.0 / 9.9      64 x 4096 x 4096: 8.1 / 11.8 against 7.0 / 9.2
-//   64x64     against 128 wide   512 x 4096 x 4096:   10.8 / 14.7  against 17.0 / 22.1
-//   128 wide  against 64x64      2048 x 4096 x 4096:  26.0 / 31.8  against 33.4 / 50.1     (E4M3: 128x256 tiles, eight waves)
-//   256x256   against 128 wide   4096 x 4096 x 4096:  42.0 / 55.1  against 47.8 / 60.4     2048 x 4096: 34.0 / 45.8 against 26.0 / 31.8
-//   a part-filled last round of 256x256 tiles (5330 x 4096 x 1024, 1.3 rounds): 31.4 / 38.7 against 30.3 / 32.2 with 128x128
+// Which form.  The products are bound by moving their operands from L2 to LDS (7 to 9 TB/s beside the matrix units) and by the clock that
+// the matrix units' power leaves: the largest tile wins that fills the chip, and where K is short, one that leaves room for a second
+// workgroup per CU, whose main loop covers the first one's epilogue.  us, fp16 out, each pair measured on one MI355X:
+//   M x N x K              E2M1                                       E4M3
+//   32 x 4096 x 4096       rows 5.7, 64x64 7.1                        rows 7.4, 64x64 9.8
+//   64 x 4096 x 4096       rows 8.8, 64x64 7.2                        rows 12.4, 64x64 10.0
+//   512 x 4096 x 4096      64x64 11.5, 128x128 17.1                   64x64 15.5, 128x256 22.6
+//   2048 x 4096 x 4096     64x64 34.7, 128x128 26.2, 256x256 32.6     64x64 50.6, 128x256 32.0, 256x256 45.9
+//   2048 x 4096 x 1024     64x64 17.6, 128x128 13.6, 256x256 15.9     64x64 19.8, 128x256 14.6, 128x128 16.2
+//   4096 x 4096 x 1024     256x256 22.8, 128x128 24.7                 256x256 25.0, 128x128 27.8
+//   5330 x 4096 x 1024     128x128 29.7 (256-wide steps 31.4)         128x128 36.7, 256x256 41.8
+//     with GELU            128x128 35.5 (256-wide steps 39.5)         128x128 40.3, 128x256 45.2
+//   21320 x 4096 x 1024    128x128 104, 256x256 119, with GELU 126, 169    133, 141, with GELU 165, 180
+//   5330 x 4096 x 4096     128x128 68.2 (128-wide steps 76.7), 256x256 72.5    128x256 87.1, 128x128 97.8, 256x256 98.5
+//   16384 x 4096 x 4096    128x128 218, 256x256 183                   128x256 292, 256x256 267
 template <int FA>
 int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
   const long t16 = (long)csam_cdiv(p.M, 16) * csam_cdiv(p.N, 16);
@@ -473,17 +481,20 @@ int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
     return CSAM_OK;
   }
   const long t256 = (long)csam_cdiv(p.M, 256) * csam_cdiv(p.N, 256), rounds = (t256 + 255) / 256;
-  const bool filled = rounds >= 4 || t256 * 4 >= rounds * 256 * 3;
+  const bool brief = p.Kp <= 1024;
+  const bool large = brief ? t256 >= 240 && rounds == 1 : rounds >= 4 || t256 * 4 >= rounds * 256 * 3;
   if constexpr (FA == CSAM_MX_FP4) {
-    if (filled) return mx_tiles<FA, 256, 256, 2, 4, 3, 128>(st, p);
-    if ((long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128) >= 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 256>(st, p);
-    return mx_tiles<FA, 64, 64, 2, 2, 3, 256>(st, p);
+    const long t128 = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128);
+    if (large) return mx_tiles<FA, 256, 256, 2, 4, 3, 128>(st, p);
+    if (t128 < 256) return mx_tiles<FA, 64, 64, 2, 2, 3, 256>(st, p);
+    if (brief && t128 > 512) return mx_tiles<FA, 128, 128, 2, 2, 2, 128>(st, p);
+    return mx_tiles<FA, 128, 128, 2, 2, 2, 256>(st, p);
   } else {
-    if (filled) return mx_tiles<FA, 256, 256, 4, 2, 3, 128>(st, p);
-    const long t128 = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 256);
-    if (t128 > 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 128>(st, p);
-    if (t128 >= 128) return mx_tiles<FA, 128, 256, 2, 4, 3, 128>(st, p);
-    return mx_tiles<FA, 64, 64, 2, 2, 3, 128>(st, p);
+    const long wide = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 256);
+    if (large) return mx_tiles<FA, 256, 256, 4, 2, 3, 128>(st, p);
+    if (wide < 128) return mx_tiles<FA, 64, 64, 2, 2, 3, 128>(st, p);
+    if (!brief || wide <= 256) return mx_tiles<FA, 128, 256, 2, 4, 3, 128>(st, p);
+    return mx_tiles<FA, 128, 128, 2, 2, 2, 128>(st, p);
   }
 }
 

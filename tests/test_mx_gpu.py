@@ -128,7 +128,8 @@ def close(out, ref, tol):
 
 SHAPES = [(1, 1, 1), (1, 16, 32), (1, 130, 256), (7, 33, 500), (15, 16, 512), (16, 250, 2048), (17, 64, 1000), (33, 31, 256),
           (64, 128, 1280), (65, 129, 256), (127, 200, 300), (130, 128, 512), (300, 384, 1280), (513, 260, 1001),
-          (1000, 1024, 256), (40, 200, 256), (2100, 2000, 256), (3333, 4001, 256), (5330, 1900, 300)]
+          (1000, 1024, 256), (40, 200, 256), (2100, 2000, 256), (3333, 4001, 256), (5330, 1900, 300),
+          (3333, 4001, 1290), (4001, 4001, 300), (2600, 4001, 1500)]
 
 
 @pytest.mark.parametrize("fa", ["fp4", "fp8"])
@@ -162,13 +163,13 @@ def test_gemm_matches_float64(cuda, fa, m, n, k):
 
 
 @pytest.mark.parametrize("fa", ["fp4", "fp8"])
-@pytest.mark.parametrize("m", [5, 70, 300, 33000])
+@pytest.mark.parametrize("m", [5, 70, 300, 33000, 65000])
 @pytest.mark.parametrize("act", [0, 1, 2])
 @pytest.mark.parametrize("out_dtype,res_dtype", [(torch.float16, None), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32),
                                                  (torch.float16, torch.float32), (torch.float32, torch.float16)])
 def test_gemm_epilogues(cuda, fa, m, act, out_dtype, res_dtype):
     from crowdsam_amd import hip
-    n, k = (200, 320) if m < 1000 else (508, 100)          # the last: 256 x 256 tiles, one row and part of a tile of columns over
+    n, k = (508, 100) if m == 33000 else (200, 320)         # 33000: 128 x 128 tiles, part of a tile of columns over; 65000: 256 x 256
     a, w = operands(m, n, k, fa, 11 + m)
     bias = torch.randn(n, generator=gen(2))
     res = None if res_dtype is None else torch.randn(m, n, generator=gen(3)).to(res_dtype)
