@@ -23,7 +23,7 @@ struct MxGemmArgs {
   const float* bias;
   const void* R; long ldr; int r_dt;
   int act, M, N, Kp;
-  int vec;                                   // N is a multiple of 4
+  int past;                                  // C's rows begin on lines of 128 bytes: large tiles may store past the caches
 };
 
 typedef const __attribute__((address_space(1))) void* gptr_t;
@@ -33,6 +33,12 @@ __device__ __forceinline__ void glds4(const void* g, void* l) { __builtin_amdgcn
 
 __device__ __forceinline__ float mx_elem(const void* p, int dt, long i) {
   return dt == CSAM_DT_F32 ? ((const float*)p)[i] : dt == CSAM_DT_F16 ? (float)((const half_t*)p)[i] : (float)((const bf16_t*)p)[i];
+}
+
+__device__ __forceinline__ void mx_put(void* p, int dt, long i, float x) {
+  if (dt == CSAM_DT_F32) ((float*)p)[i] = x;
+  else if (dt == CSAM_DT_F16) ((half_t*)p)[i] = (half_t)x;
+  else ((bf16_t*)p)[i] = (bf16_t)x;
 }
 
 // GELU, as csam_gemm_f16 computes it: the erf form where the result stays fp32, for 16-bit results the polynomial of Phi (off by 6.5e-5 at
@@ -95,21 +101,26 @@ __device__ __forceinline__ void mx_epilogue4(const MxGemmArgs& p, int m, int n, 
     if (n + i < p.N) {
       float x = v[i];
       if (p.R) x += mx_elem(p.R, p.r_dt, (long)m * p.ldr + n + i);
-      const long at = (long)m * p.ldc + n + i;
-      if (p.c_dt == CSAM_DT_F32) ((float*)p.C)[at] = x;
-      else if (p.c_dt == CSAM_DT_F16) ((half_t*)p.C)[at] = (half_t)x;
-      else ((bf16_t*)p.C)[at] = (bf16_t)x;
+      mx_put(p.C, p.c_dt, (long)m * p.ldc + n + i, x);
     }
   }
 }
 
-// (the large tiles' results go past the caches: 16384 x 4096 x 4096 185 us, 170 so; 5330 x 4096 x 1024 with GELU 37.6, 35.9)
-// 4 consecutive columns of B rows STEP apart, all four inside N or none; every choice is uniform and made once for the B rows
+// The large tiles' results go past the caches where every line of C belongs to one wave (16384 x 4096 x 4096 185 us, 170 so; 5330 x 4096 x
+// 1024 with GELU 37.6, 35.9); lines that waves share have to meet in the L2 (6312 x 3178 x 206 28.2 us, past the caches 40.3).
+// 4 consecutive columns of B rows STEP apart; every choice is uniform and made once for the B rows, but for the `left` < 4 last columns of
+// rows whose length is no multiple of 4
 template <int B, int STEP, bool NT>
 __device__ __forceinline__ void mx_epilogue_rows(const MxGemmArgs& p, int m, int n, floatx4 bz, floatx4 (&v)[B]) {
   if (n >= p.N) return;
+  const int left = p.N - n;
   floatx4 res[B];
-  if (p.R) {
+  if (p.R && left < 4) {
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) res[b][i] = m + b * STEP < p.M && i < left ? mx_elem(p.R, p.r_dt, (long)(m + b * STEP) * p.ldr + n + i) : 0.f;
+  } else if (p.R) {
     const long at = (long)m * p.ldr + n;
     if (p.r_dt == CSAM_DT_F32) {
 #pragma unroll
@@ -145,10 +156,20 @@ __device__ __forceinline__ void mx_epilogue_rows(const MxGemmArgs& p, int m, int
 #pragma unroll
     for (int b = 0; b < B; ++b) v[b] += res[b];
   }
+  if (left < 4) {
 #pragma unroll
-  for (int b = 0; b < B; ++b) {
-    if (m + b * STEP >= p.M) return;
-    mx_store4<NT>(p.C, p.c_dt, (long)(m + b * STEP) * p.ldc + n, v[b]);
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (m + b * STEP < p.M && i < left) mx_put(p.C, p.c_dt, (long)(m + b * STEP) * p.ldc + n + i, v[b][i]);
+  } else if (NT && p.past) {
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (m + b * STEP < p.M) mx_store4<true>(p.C, p.c_dt, (long)(m + b * STEP) * p.ldc + n, v[b]);
+  } else {
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (m + b * STEP < p.M) mx_store4(p.C, p.c_dt, (long)(m + b * STEP) * p.ldc + n, v[b]);
   }
 }
 
@@ -366,7 +387,12 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
   constexpr int LPR = COLS / 4, RPI = 64 / LPR, B = 4;     // lanes of a row, rows of an access, accesses of a batch
   float* buf = (float*)smem + wave * 32 * PITCH;
   const int n = bn0 + wn * COLS + (lane % LPR) * 4, mr = bm0 + wm * MI * 32 + lane / LPR;
-  const floatx4 bz = p.vec && p.bias && n < p.N ? mx_load4(p.bias, CSAM_DT_F32, n) : floatx4{0.f, 0.f, 0.f, 0.f};
+  floatx4 bz = {0.f, 0.f, 0.f, 0.f};
+  if (p.bias && n + 4 <= p.N) bz = mx_load4(p.bias, CSAM_DT_F32, n);
+  else if (p.bias)
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (n + j < p.N) bz[j] = p.bias[n + j];
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -376,17 +402,12 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
         *(floatx4*)(buf + r * PITCH + j * 32 + 8 * e + 4 * g) =
             floatx4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
     const float* src = buf + lane / LPR * PITCH + (lane % LPR) * 4;
-    if (p.vec) {                                           // N is a multiple of 4: a lane's four columns are inside or outside together
 #pragma unroll 1
-      for (int s = 0; s < 32 / RPI; s += B) {
-        floatx4 v[B];
+    for (int s = 0; s < 32 / RPI; s += B) {
+      floatx4 v[B];
 #pragma unroll
-        for (int b = 0; b < B; ++b) v[b] = *(const floatx4*)(src + (s + b) * RPI * PITCH);
-        mx_epilogue_rows<B, RPI, (TM >= 128)>(p, mr + i * 32 + s * RPI, n, bz, v);
-      }
-    } else {
-#pragma unroll 1
-      for (int s = 0; s < 32 / RPI; ++s) mx_epilogue4(p, mr + i * 32 + s * RPI, n, *(const floatx4*)(src + s * RPI * PITCH));
+      for (int b = 0; b < B; ++b) v[b] = *(const floatx4*)(src + (s + b) * RPI * PITCH);
+      mx_epilogue_rows<B, RPI, (TM >= 128)>(p, mr + i * 32 + s * RPI, n, bz, v);
     }
   }
 }
@@ -460,9 +481,10 @@ int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
 // the matrix units' power leaves: the largest tile wins that fills the chip, and where K is short, one that leaves room for a second
 // workgroup per CU, whose main loop covers the first one's epilogue.  us, fp16 out, each pair measured on one MI355X:
 //   M x N x K              E2M1                                       E4M3
-//   32 x 4096 x 4096       rows 5.7, 64x64 7.1                        rows 7.4, 64x64 9.8
-//   64 x 4096 x 4096       rows 8.8, 64x64 7.2                        rows 12.4, 64x64 10.0
-//   512 x 4096 x 4096      64x64 11.5, 128x128 17.1                   64x64 15.5, 128x256 22.6
+//   32 x 4096 x 4096       rows 5.7, 64x64 6.7                        rows 7.5, 64x64 7.8
+//   224 x 4096 x 4096      64x64 7.8 (three stages 8.2), 128x64 10.2  64x64 9.2 (three stages 10.9), 64x128 11.4
+//   512 x 4096 x 4096      64x64 11.7, 128x64 11.0, 128x128 16.8      64x64 15.3, 64x128 12.9, 128x256 22.0
+//   1330 x 1024 x 4096     64x64 10.3, 128x64 10.1, 128x128 16.6      64x64 14.1, 64x128 11.8, 128x256 22.0
 //   2048 x 4096 x 4096     64x64 34.7, 128x128 26.2, 256x256 32.6     64x64 50.6, 128x256 32.0, 256x256 45.9
 //   2048 x 4096 x 1024     64x64 17.6, 128x128 13.6, 256x256 15.9     64x64 19.8, 128x256 14.6, 128x128 16.2
 //   4096 x 4096 x 1024     256x256 22.8, 128x128 24.7                 256x256 25.0, 128x128 27.8
@@ -486,13 +508,17 @@ int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
   if constexpr (FA == CSAM_MX_FP4) {
     const long t128 = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128);
     if (large) return mx_tiles<FA, 256, 256, 2, 4, 3, 128>(st, p);
-    if (t128 < 256) return mx_tiles<FA, 64, 64, 2, 2, 3, 256>(st, p);
+    if (t128 < 256) return mx_tiles<FA, 64, 64, 2, 2, 4, 256>(st, p);
     if (brief && t128 > 512) return mx_tiles<FA, 128, 128, 2, 2, 2, 128>(st, p);
     return mx_tiles<FA, 128, 128, 2, 2, 2, 256>(st, p);
   } else {
     const long wide = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 256);
     if (large) return mx_tiles<FA, 256, 256, 4, 2, 3, 128>(st, p);
-    if (wide < 128) return mx_tiles<FA, 64, 64, 2, 2, 3, 128>(st, p);
+    if (wide < 128) {
+      const int n64 = csam_cdiv(p.N, 64), n128 = csam_cdiv(p.N, 128);       // (N = 137: 64x64 23.0, 64x128, half of it empty, 27.6)
+      if ((long)csam_cdiv(p.M, 64) * n64 <= 256 || n128 * 15 > n64 * 8) return mx_tiles<FA, 64, 64, 2, 2, 4, 128>(st, p);
+      return mx_tiles<FA, 64, 128, 2, 2, 4, 128>(st, p);
+    }
     if (!brief || wide <= 256) return mx_tiles<FA, 128, 256, 2, 4, 3, 128>(st, p);
     return mx_tiles<FA, 128, 128, 2, 2, 2, 128>(st, p);
   }
@@ -520,6 +546,6 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
                "csam_mx_gemm: scale groups have to lie 4-byte aligned, at least 4 * rows bytes apart");
   CSAM_REQUIRE(ldc >= N && (!residual || ldr >= N), "csam_mx_gemm: an output row pitch is shorter than N");
   MxGemmArgs p = {(const uint8_t*)A, lda, (const uint8_t*)A_scales, a_scale_stride, (const uint8_t*)W, ldw, (const uint8_t*)W_scales,
-                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act, M, N, Kp, N % 4 == 0};
+                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act, M, N, Kp, al(C, ldc * (c_dtype == CSAM_DT_F32 ? 4 : 2), 128)};
   return a_fmt == CSAM_MX_FP8 ? mx_gemm_launch<CSAM_MX_FP8>((hipStream_t)stream, p) : mx_gemm_launch<CSAM_MX_FP4>((hipStream_t)stream, p);
 }

@@ -12,10 +12,10 @@ struct RotaryArgs {
   const double* freq; const int* axis;              // [P] radians per unit, axis of each pair
   int T, Tp, Hq, Hk, hd, P, axes;
   int tokens, heads, splits;                        // tokens and heads of a workgroup, workgroups that share a token's heads
-  int units, Pp;                                    // units of a head; P rounded up to whole 16-byte table reads
+  int units, turning, Pp;                           // units of a head, those that rotate (half); P rounded up to whole units' table reads
   unsigned by_unit, by_token, by_pair;              // ceil(2^32 / d) for d = units, heads * units, P
 };
-constexpr int ROT_TABLE = 2048;                     // (cos, sin) entries of a workgroup's table: 16 KB
+constexpr int ROT_TABLE = 2048;                     // (cos, sin) entries of a workgroup's table: 16 KB (and one unit's over)
 
 // n / d by d's reciprocal: exact while n * d < 2^32, and every n here is below 2^16
 __device__ __forceinline__ unsigned rot_div(unsigned n, unsigned r, int d) { return d == 1 ? n : __umulhi(n, r); }
@@ -43,20 +43,57 @@ __device__ __forceinline__ float2_t rotary_angle(const RotaryArgs& p, int t, int
 // units, HB of a thread's at a time, the first of them fetched before the angles are computed:
 //   half:        VW elements of the first half of the pairs and their VW partners, or VW elements that pass through;
 //   interleaved: VW consecutive elements = VW / 2 pairs.
+// What is left of a run of the head behind its whole units (PIECES) is units of VW / 2, VW / 4, .. 1 elements, as its length has bits
+// (16384 tokens x 32 heads of 64 with 17 pairs, half, fp16: 48.0 us; with accesses of one element throughout 93.3).
 // Consecutive threads hold consecutive units of a head, then the next head: a wave touches whole runs of the row.
-template <typename T, bool HALF, int VW, bool NT>
+template <int VW>
+__device__ __forceinline__ int rotary_unit(int u, int n, int& size) {         // unit u of a run of n elements: where it begins, its size
+  const int whole = n / VW, j = u - whole;
+  size = VW;
+  if (j < 0) return u * VW;
+  int at = whole * VW, k = 0;
+#pragma unroll
+  for (int s = VW / 2, found = 0; s; s >>= 1) {
+    const bool bit = n & s, mine = bit && k == j;
+    if (mine) size = s, found = 1;
+    at += bit && !found ? s : 0;
+    k += bit;
+  }
+  return at;
+}
+template <typename T, int VW, int N>
+__device__ __forceinline__ void rotary_take(const T* p, int size, typename csam_pack<T, VW>::vec& v) {
+  if (size == N) {
+    const auto h = *(const typename csam_pack<T, N>::at*)p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = h[i];
+  }
+  if constexpr (N > 1) rotary_take<T, VW, N / 2>(p, size, v);
+}
+template <typename T, int VW, int N, bool NT>
+__device__ __forceinline__ void rotary_give(T* p, int size, const typename csam_pack<T, VW>::vec& v) {
+  if (size == N) {
+    typename csam_pack<T, N>::vec h;
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = v[i];
+    csam_put<NT>((typename csam_pack<T, N>::at*)p, h);
+  }
+  if constexpr (N > 1) rotary_give<T, VW, N / 2, NT>(p, size, v);
+}
+
+template <typename T, bool HALF, int VW, bool PIECES, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
   typedef typename csam_pack<T, VW>::vec vec_t;
   typedef typename csam_pack<T, VW>::at vec_at;
   constexpr int HB = 4, NP = HALF ? VW : VW / 2;
-  __shared__ __attribute__((aligned(16))) float2_t table[ROT_TABLE];
+  __shared__ __attribute__((aligned(16))) float2_t table[ROT_TABLE + NP];
   const int hb = blockIdx.x % p.splits * p.heads;
   const int t0 = (int)(blockIdx.x / p.splits) * p.tokens, nt = min(p.tokens, p.T - t0);
   const int H = p.Hq + p.Hk, per_token = p.heads * p.units, total = nt * per_token;
 
   vec_t v[HB], w[HB];
   T* dst[HB];                                       // where the unit goes; null: no unit
-  short pair0[HB], tl[HB];
+  short pair0[HB], tl[HB], size[HB];                // its first pair, token and elements
   auto fetch = [&](int first) {
 #pragma unroll
     for (int b = 0; b < HB; ++b) {
@@ -67,16 +104,29 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
       const int h = hb + hl;
       if (h >= H) continue;
       const long t = t0 + tk;
-      pair0[b] = (short)(u * NP);
+      const bool turn = !HALF || u < p.turning;     // of a half layout's units, the first `turning` rotate, the others pass through
+      int i0, sz = VW;
+      if constexpr (PIECES) i0 = turn ? rotary_unit<VW>(u, HALF ? p.P : p.hd, sz) : rotary_unit<VW>(u - p.turning, p.hd - 2 * p.P, sz);
+      else i0 = (turn ? u : u - p.turning) * VW;
+      pair0[b] = (short)(turn ? (HALF ? i0 : i0 >> 1) : p.P);
+      if (!turn) i0 += 2 * p.P;
       tl[b] = (short)tk;
-      const int i0 = HALF && u * NP >= p.P ? u * VW + p.P : u * VW;
+      size[b] = (short)sz;
       const bool isq = h < p.Hq;
       const T* src = (isq ? (const T*)p.q + t * p.ldq + (long)h * p.hsq : (const T*)p.k + t * p.ldk + (long)(h - p.Hq) * p.hsk) + i0;
       dst[b] = (isq ? (T*)p.qo + t * p.ldqo + (long)h * p.hsqo : (T*)p.ko + t * p.ldko + (long)(h - p.Hq) * p.hsko) + i0;
-      if (!HALF && VW == 2 && i0 + 1 == p.hd) v[b][0] = src[0];            // the last element of a head of odd width
-      else v[b] = *(const vec_at*)src;
-      if (HALF && u * NP < p.P) w[b] = *(const vec_at*)(src + p.P);
+      if constexpr (PIECES) {
+        rotary_take<T, VW, VW>(src, sz, v[b]);
+        if (HALF && turn) rotary_take<T, VW, VW>(src + p.P, sz, w[b]);
+      } else {
+        v[b] = *(const vec_at*)src;
+        if (HALF && turn) w[b] = *(const vec_at*)(src + p.P);
+      }
     }
+  };
+  auto store = [&](T* to, int sz, const vec_t& x) {
+    if constexpr (PIECES) rotary_give<T, VW, VW, NT>(to, sz, x);
+    else csam_put<NT>((vec_at*)to, x);
   };
   fetch(threadIdx.x);
   for (int i = threadIdx.x; i < nt * p.P; i += 256) {
@@ -90,7 +140,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
     for (int b = 0; b < HB; ++b) {
       if (!dst[b]) continue;
       const bool turn = pair0[b] < p.P;
-      float2_t cs[NP];
+      float2_t cs[NP];                              // (entries behind the last pair are read and not used)
       if (turn) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) cs[i] = table[tl[b] * p.Pp + pair0[b] + i];
@@ -103,9 +153,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
             v[b][i] = (T)(x * cs[i][0] - y * cs[i][1]);
             w[b][i] = (T)(x * cs[i][1] + y * cs[i][0]);
           }
-          csam_put<NT>((vec_at*)(dst[b] + p.P), w[b]);
+          store(dst[b] + p.P, size[b], w[b]);
         }
-        csam_put<NT>((vec_at*)dst[b], v[b]);
       } else {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -115,18 +164,22 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
             v[b][2 * i + 1] = (T)(x * cs[i][1] + y * cs[i][0]);
           }
         }
-        if (VW == 2 && pair0[b] * 2 + 1 == p.hd) dst[b][0] = v[b][0];
-        else csam_put<NT>((vec_at*)dst[b], v[b]);
       }
+      store(dst[b], size[b], v[b]);
     }
   }
 }
 
-template <typename T, bool HALF, int VW>
-int rotary_go(hipStream_t st, RotaryArgs& p) {
-  constexpr int NP = HALF ? VW : VW / 2, HB = 4;
-  p.units = csam_cdiv(HALF ? p.hd - p.P : p.hd, VW);
-  p.Pp = csam_cdiv(p.P, NP > 2 ? NP : 2) * (NP > 2 ? NP : 2);
+// the widest accesses, at any element's address
+template <typename T, bool HALF>
+int rotary_launch(hipStream_t st, RotaryArgs& p) {
+  constexpr int VW = 16 / sizeof(T), NP = HALF ? VW : VW / 2, HB = 4;
+  const int rest = p.hd - 2 * p.P;
+  const bool pieces = HALF ? p.P % VW || rest % VW : p.hd % VW;
+  auto units = [](int n) { return n / VW + __builtin_popcount((unsigned)n % VW); };
+  p.turning = HALF ? units(p.P) : 0;
+  p.units = HALF ? p.turning + units(rest) : units(p.hd);
+  p.Pp = csam_cdiv(p.P, NP) * NP;
   const int H = p.Hq + p.Hk;
   // A workgroup's units: one batch of its threads (16384 tokens x 32 heads of 80: 39.8 us, 45.4 with two batches).  A token with more is
   // shared by workgroups, tokens with fewer share one; a call that would not give every CU a workgroup this way is cut finer.
@@ -140,22 +193,18 @@ int rotary_go(hipStream_t st, RotaryArgs& p) {
   p.by_pair = recip(p.P);
   const long grid = (long)csam_cdiv(p.T, p.tokens) * p.splits;
   CSAM_REQUIRE(grid < (1L << 31), "csam_rotary: too many elements");
-  // results beyond the L2s' size are stored past them (the same call: 39.8 us, 33.0 so)
-  if (all * VW * (long)sizeof(T) > (32L << 20)) rotary_kernel<T, HALF, VW, true><<<(unsigned)grid, 256, 0, st>>>(p);
-  else rotary_kernel<T, HALF, VW, false><<<(unsigned)grid, 256, 0, st>>>(p);
+  // Results beyond the L2s' size are stored past them (16384 tokens x 32 heads of 80, interleaved: 30.6 us, 27.7 so; of 128 with 64 pairs,
+  // half: 53.5, 42.1), unless a run of a head ends inside a 64-byte line, which two stores then fill: those meet in the L2 (of 80 with 40
+  // pairs, half: past the caches 61.8, 32.2 so).
+  const bool lines = !HALF || (p.P * sizeof(T) % 64 == 0 && rest * sizeof(T) % 64 == 0);
+  const bool past = lines && (long)p.T * H * p.hd * (long)sizeof(T) > (32L << 20);
+  if (pieces && past) {                              // (half layouts of whole lines have no pieces)
+    if constexpr (!HALF) rotary_kernel<T, HALF, VW, true, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  } else if (pieces) rotary_kernel<T, HALF, VW, true, false><<<(unsigned)grid, 256, 0, st>>>(p);
+  else if (past) rotary_kernel<T, HALF, VW, false, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  else rotary_kernel<T, HALF, VW, false, false><<<(unsigned)grid, 256, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_rotary");
   return CSAM_OK;
-}
-
-// the widest accesses that units of whole accesses allow (addresses need no alignment beyond an element's)
-template <typename T>
-int rotary_launch(hipStream_t st, RotaryArgs& p, int half) {
-  constexpr int W = 16 / sizeof(T);
-  const int odd = half ? p.P | p.hd : p.hd;
-  if (odd % W == 0) return half ? rotary_go<T, true, W>(st, p) : rotary_go<T, false, W>(st, p);
-  if (W == 8 && odd % 4 == 0) return half ? rotary_go<T, true, 4>(st, p) : rotary_go<T, false, 4>(st, p);
-  if (!half) return rotary_go<T, false, 2>(st, p);
-  return odd % 2 == 0 ? rotary_go<T, true, 2>(st, p) : rotary_go<T, true, 1>(st, p);
 }
 
 }  // namespace
@@ -174,9 +223,9 @@ extern "C" int csam_rotary(void* stream, const void* q, long ldq, int hsq, void*
   CSAM_REQUIRE(dtype == CSAM_DT_F16 || dtype == CSAM_DT_F32 || dtype == CSAM_DT_BF16, "csam_rotary: bad dtype %d", dtype);
   CSAM_REQUIRE(hsq >= head_dim && hsqo >= head_dim && (!Hk || (hsk >= head_dim && hsko >= head_dim)), "csam_rotary: heads overlap");
   RotaryArgs p = {q, q_out, ldq, ldqo, Hk ? k : nullptr, Hk ? k_out : nullptr, ldk, ldko, hsq, hsqo, hsk, hsko, pos, pos_stride, pos_is_f32,
-                  freq, axis, T, T_pos, Hq, Hk, head_dim, pairs, axes, 0, 0, 0, 0, 0, 0, 0, 0};
+                  freq, axis, T, T_pos, Hq, Hk, head_dim, pairs, axes};
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CSAM_DT_F16) return rotary_launch<half_t>(st, p, !interleaved);
-  if (dtype == CSAM_DT_BF16) return rotary_launch<bf16_t>(st, p, !interleaved);
-  return rotary_launch<float>(st, p, !interleaved);
+  if (dtype == CSAM_DT_F16) return interleaved ? rotary_launch<half_t, false>(st, p) : rotary_launch<half_t, true>(st, p);
+  if (dtype == CSAM_DT_BF16) return interleaved ? rotary_launch<bf16_t, false>(st, p) : rotary_launch<bf16_t, true>(st, p);
+  return interleaved ? rotary_launch<float, false>(st, p) : rotary_launch<float, true>(st, p);
 }
