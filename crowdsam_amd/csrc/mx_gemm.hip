@@ -12,6 +12,7 @@
 // W rows are the instruction's row operand, A rows its columns: a lane ends up with 4 consecutive n of one row m.
 #include <type_traits>
 #include <utility>
+#include <limits.h>
 #include "mx_common.h"
 
 namespace {
@@ -532,6 +533,7 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
   if (M == 0 || N == 0) return CSAM_OK;
   CSAM_REQUIRE(A && A_scales && W && W_scales && C, "csam_mx_gemm: null operand");
   CSAM_REQUIRE(M > 0 && N > 0 && K > 0, "csam_mx_gemm: bad sizes M %d N %d K %d", M, N, K);
+  CSAM_REQUIRE(M <= INT_MAX - 255 && N <= INT_MAX - 255, "csam_mx_gemm: %d x %d is over 2^31 - 256 rows or columns", M, N);
   CSAM_REQUIRE(a_fmt == CSAM_MX_FP4 || a_fmt == CSAM_MX_FP8, "csam_mx_gemm: bad format %d", a_fmt);
   CSAM_REQUIRE(K <= (1 << 20), "csam_mx_gemm: K %d is over 2^20", K);
   const int Kp = csam_cdiv(K, 256) * 256;

@@ -1,5 +1,6 @@
 // Quantisation to and from microscaled (MX) operands, and the root-mean-square norm that can hand its rows out as one.
 // All of it is bound by memory: a pass reads each input once and writes each output once.
+#include <limits.h>
 #include <type_traits>
 #include "mx_common.h"
 
@@ -203,6 +204,7 @@ bool dt_ok(int dt) { return dt == CSAM_DT_F16 || dt == CSAM_DT_F32 || dt == CSAM
 int mx_check(const char* who, const void* codes, long ldc, const void* scales, long sstride, int fmt, int M, int K) {
   CSAM_REQUIRE(codes && scales, "%s: null operand", who);
   CSAM_REQUIRE(fmt == CSAM_MX_FP4 || fmt == CSAM_MX_FP8, "%s: format %d is neither CSAM_MX_FP4 nor CSAM_MX_FP8", who, fmt);
+  CSAM_REQUIRE(M <= INT_MAX - 255 && K <= INT_MAX - 255, "%s: %d x %d is over 2^31 - 256 rows or columns", who, M, K);
   const long Kp = (K + 255L) / 256 * 256;
   CSAM_REQUIRE(ldc >= (fmt == CSAM_MX_FP4 ? Kp / 2 : Kp), "%s: code rows of %ld bytes are shorter than %ld padded columns", who, ldc, Kp);
   CSAM_REQUIRE(aligned(codes, ldc, 16), "%s: codes and their row pitch have to be multiples of 16 bytes", who);

@@ -1218,7 +1218,7 @@ def _mx_check(q, who, name):
     if c.dtype != torch.uint8 or s.dtype != torch.uint8:
         raise ValueError(f"{who}: {name} has {c.dtype} codes and {s.dtype} scales, not uint8")
     shape = c.shape
-    if len(shape) != 2 or shape[1] != width or shape[0] > _INT_MAX:
+    if len(shape) != 2 or shape[1] != width or shape[0] > _INT_MAX - 255:
         raise ValueError(f"{who}: {name} has codes of shape {tuple(shape)}, not [rows, {width}] (K = {K} padded to {Kp})")
     rows = shape[0]
     if s.shape != (Kp // 128, rows, 4):
@@ -1294,6 +1294,8 @@ def mx_quantize(x, fmt="fp4"):
     M, K = x.shape
     if K == 0:
         raise ValueError("mx_quantize: x has no columns")
+    if max(M, K) > _INT_MAX - 255:
+        raise ValueError(f"mx_quantize: {M} x {K} is over 2^31 - 256 rows or columns")
     dev = _same_device("mx_quantize", x)
     q = _mx_empty(x, M, K, fmt)
     _call_on(dev, "csam_mx_quantize", x.data_ptr(), ld, _DT3[x.dtype], q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), 4 * M,
@@ -1315,7 +1317,7 @@ def mx_dequantize(q, out_dtype=torch.float32):
 
 def mx_gemm(a, w, out=None, bias=None, act=ACT_NONE, residual=None, out_dtype=torch.float16):
     """out[M, N] = act(a w^T + bias) + residual of two ``MxTensor``s: ``a`` [M, K] in "fp4" or "fp8", ``w`` [N, K] in "fp4"; fp32 sums,
-    rounded once.  ``bias`` fp32 [N]; ``residual`` [M, N] fp16 / bfloat16 / fp32; ``out`` may be the residual.  The kernel and with it the
+    rounded once to ``out``'s type or ``out_dtype``.  ``bias`` fp32 [N]; ``residual`` [M, N] fp16 / bfloat16 / fp32; ``out`` may be the residual.  The kernel and with it the
     order of the sum depend on the sizes: rows are not bitwise independent of M."""
     who = "mx_gemm"
     if w.fmt != "fp4":

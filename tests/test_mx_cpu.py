@@ -34,6 +34,7 @@ def test_reference_rounds_ties_to_even_and_saturates():
     (lambda: hip.mx_quantize(torch.zeros(4, 0)), "no columns"),
     (lambda: hip.mx_quantize(torch.zeros(32)), "dimensions"),
     (lambda: hip.mx_quantize(torch.zeros(32, 4).t()), "not contiguous"),
+    (lambda: hip.mx_quantize(torch.empty(1, (1 << 31) - 100, dtype=torch.float16, device="meta")), "columns"),
     (lambda: hip.mx_quantize(torch.zeros(1, 32).expand(4, 32)), "overlap"),
     (lambda: hip.mx_quantize(torch.zeros(4, 32)), "no CPU form"),
     (lambda: hip.mx_dequantize(mx(4, 100, "fp4"), torch.int32), "int32"),
@@ -107,6 +108,9 @@ def test_entries_check_for_themselves():
     assert lib.csam_mx_quantize(None, None, 0, 0, None, 0, None, 0, 0, 1, 1) == -1 and b"null" in lib.csam_last_error()
     assert lib.csam_mx_quantize(None, 64, 32, 0, 64, 128, 64, 4, 2, 1, 32) == -1 and b"format" in lib.csam_last_error()
     assert lib.csam_mx_quantize(None, 64, 32, 0, 64, 120, 64, 4, 0, 1, 32) == -1 and b"padded" in lib.csam_last_error()
+    assert lib.csam_mx_quantize(None, 64, 1, 0, 64, 128, 64, 1 << 33, 0, (1 << 31) - 1, 1) == -1 and b"2^31" in lib.csam_last_error()
+    assert lib.csam_mx_gemm(None, 64, 128, 64, 1 << 33, 0, 64, 128, 64, 4, 64, 1, 0, None, None, 0, 0, 0, (1 << 31) - 1, 1, 32) == -1 and \
+        b"2^31" in lib.csam_last_error()
     assert lib.csam_mx_dequantize(None, 64, 128, 64, 4, 0, 64, 31, 0, 1, 32) == -1 and b"sizes" in lib.csam_last_error()
     assert lib.csam_mx_gemm(None, 64, 128, 64, 4, 0, 72, 128, 64, 4, 64, 1, 0, None, None, 0, 0, 0, 1, 1, 32) == -1 and b"16 bytes" in lib.csam_last_error()
     assert lib.csam_rms_norm(None, 64, 8, 0, 64, 8, 0, None, 8, 64, 1e-6, 64, 8, 0, 1, 8) == -1 and b"together" in lib.csam_last_error()

@@ -231,6 +231,20 @@ def test_gemm_large_offsets(cuda):
     assert torch.equal(out[:130], hip.mx_gemm(qa.rows(0, 130), qw, out_dtype=torch.bfloat16))
 
 
+@pytest.mark.parametrize("fa", ["fp4", "fp8"])
+@pytest.mark.parametrize("m", [2, 70])
+def test_gemm_longest_rows(cuda, fa, m):
+    """K = 2^20, and one more is refused.  Every value is a power of two and a row of A has one sign, so the sums stay exact."""
+    from crowdsam_amd import hip
+    n, k = 130, 1 << 20
+    sign = torch.where(torch.arange(m) % 2 == 0, 1.0, -1.0).view(m, 1).to(cuda)
+    scale = torch.exp2((torch.arange(n) % 3).float()).view(n, 1).to(cuda)
+    qa, qw = hip.mx_quantize((sign * torch.ones(m, k, device=cuda)).half(), fa), hip.mx_quantize((scale * torch.ones(n, k, device=cuda)).half(), "fp4")
+    assert torch.equal(hip.mx_gemm(qa, qw, out_dtype=torch.float32), (sign * k) @ scale.t())
+    with pytest.raises(ValueError, match="2\\^20"):
+        hip.mx_gemm(hip.mx_quantize(torch.ones(1, k + 1, device=cuda), fa), hip.mx_quantize(torch.ones(1, k + 1, device=cuda), "fp4"))
+
+
 def test_streams_and_graph_replays(cuda):
     """The four operators as a run on a stream of their own and captured; each replay is checked against the eager result."""
     from crowdsam_amd import hip

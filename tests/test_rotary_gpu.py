@@ -48,7 +48,8 @@ def positions(A, T, kind, seed):
 @pytest.mark.parametrize("T,Hq,Hk,hd,sections", [(1, 16, 16, 64, (16, 16)), (1, 1, 0, 2, (1,)), (5, 3, 1, 80, (12, 14, 14)), (70, 4, 4, 80, (12, 12, 12)),
                                                  (33, 2, 1, 64, (8,)), (17, 5, 2, 36, (9, 8)), (9, 24, 6, 128, (16, 24, 24)), (3, 2, 2, 250, (60, 50)),
                                                  (258, 1, 1, 16, (4, 4)), (4, 3, 0, 7, (2, 1)), (13, 20, 0, 250, (23,)), (9, 5, 5, 250, (20, 20, 13)),
-                                                 (40, 18, 18, 36, (11,)), (6, 2, 2, 97, (7, 8)), (5, 1, 2, 31, (15,)), (2000, 24, 24, 250, (61, 62))])
+                                                 (40, 18, 18, 36, (11,)), (6, 2, 2, 97, (7, 8)), (5, 1, 2, 31, (15,)), (2000, 24, 24, 250, (61, 62)), (3, 2, 1, 4096, (1024, 1024)),
+                                                 (2, 1, 1, 4095, (2047,))])
 def test_matches_float64(cuda, dtype, interleaved, T, Hq, Hk, hd, sections):
     from crowdsam_amd import hip
     g = torch.Generator().manual_seed(T + hd)
