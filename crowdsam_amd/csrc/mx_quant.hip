@@ -36,40 +36,64 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
   }
 }
 
-template <int FMT>
-__device__ __forceinline__ void mx_values8(const uint8_t* codes, float scale, float (&v)[8]) {
+// values of V = 4 or 8 consecutive codes, times their block's scale
+template <int FMT, int V>
+__device__ __forceinline__ void mx_values(const uint8_t* codes, float scale, float (&v)[V]) {
+  float2_t w[V / 2];
   if constexpr (FMT == CSAM_MX_FP4) {
-    const unsigned q = *(const unsigned*)codes;
-    const float2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
-    const float2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
-    const float w[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = w[i] * scale;
+    unsigned q;
+    if constexpr (V == 8) q = *(const unsigned*)codes;
+    else q = *(const unsigned short*)codes;
+    w[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0);
+    w[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+    if constexpr (V == 8) {
+      w[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2);
+      w[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+    }
   } else {
-    const uintx2 q = *(const uintx2*)codes;
-    const float2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(q[0], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q[0], true);
-    const float2_t c = __builtin_amdgcn_cvt_pk_f32_fp8(q[1], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(q[1], true);
-    const float w[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    unsigned q[V / 4];
+    if constexpr (V == 8) {
+      const uintx2 d = *(const uintx2*)codes;
+      q[0] = d[0], q[1] = d[1];
+    } else q[0] = *(const unsigned*)codes;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = w[i] * scale;
+    for (int i = 0; i < V / 4; ++i) {
+      w[2 * i] = __builtin_amdgcn_cvt_pk_f32_fp8(q[i], false);
+      w[2 * i + 1] = __builtin_amdgcn_cvt_pk_f32_fp8(q[i], true);
+    }
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = w[i / 2][i % 2] * scale;
 }
 
-template <typename T, int FMT, int R>
+// The same segments of 256 columns, a lane's V elements one 16-byte store (fp32: 20000 x 4096 from E2M1 118 us with two stores of a lane
+// side by side, 55.0 so).  NT: results that the L2s would not hold go past them if their rows are whole lines (fp16: the same operand
+// 38.0 us, 31.6 so; rows of 4100: 45.4, past the caches 59.3).
+template <typename T, int FMT, int R, bool NT>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes, long ldc, const uint8_t* __restrict__ scales,
                                                             long sstride, T* __restrict__ y, long ldy, int M, int K, int nseg) {
-  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * (8 * R) + (threadIdx.x >> 5);
-  const int c8 = seg * (Q_COLS / 8) + (threadIdx.x & 31), k = c8 * 8;
+  constexpr int V = 16 / sizeof(T), LANES = Q_COLS / V, ROWS = 256 / LANES;
+  const int seg = blockIdx.x % nseg, r0 = (blockIdx.x / nseg) * (ROWS * R) + threadIdx.x / LANES;
+  const int k = seg * Q_COLS + threadIdx.x % LANES * V;
   if (k >= K) return;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int row = r0 + 8 * i;
+    const int row = r0 + ROWS * i;
     if (row >= M) continue;
-    const unsigned s = scales[(long)(c8 >> 4) * sstride + (long)row * 4 + ((c8 >> 2) & 3)];
-    float v[8];
-    mx_values8<FMT>(codes + row * ldc + (long)c8 * (FMT == CSAM_MX_FP4 ? 4 : 8), csam_e8m0(s), v);
-    if (k + 8 <= K) csam_store8(y + (long)row * ldy + k, v);
-    else csam_store8_tail(y + (long)row * ldy + k, K - k, v);
+    const unsigned s = scales[(long)(k >> 7) * sstride + (long)row * 4 + ((k >> 5) & 3)];
+    float v[V];
+    mx_values<FMT, V>(codes + row * ldc + (FMT == CSAM_MX_FP4 ? k / 2 : k), csam_e8m0(s), v);
+    T* to = y + (long)row * ldy + k;
+    if (k + V <= K) {
+      typename csam_pack<T, V>::vec h;
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[e] = (T)v[e];
+      csam_put<NT>((typename csam_pack<T, V>::at*)to, h);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (k + e < K) to[e] = (T)v[e];
+    }
   }
 }
 
@@ -257,12 +281,16 @@ int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void
   if (int rc = mx_check("csam_mx_dequantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
   const int nseg = csam_cdiv(K, Q_COLS);
   const long grid = (long)nseg * csam_cdiv(M, 8);
-  CSAM_REQUIRE(grid < (1L << 31), "csam_mx_dequantize: too many elements");
+  CSAM_REQUIRE(2 * grid < (1L << 31), "csam_mx_dequantize: too many elements");
   hipStream_t st = (hipStream_t)stream;
 #define GO(T, F)                                                                                                         \
   do {                                                                                                                   \
-    if (grid >= 2048) mx_dequantize_kernel<T, F, 4><<<(unsigned)((long)nseg * csam_cdiv(M, 32)), 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
-    else mx_dequantize_kernel<T, F, 1><<<(unsigned)grid, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
+    constexpr int ROWS = sizeof(T) == 4 ? 4 : 8;                                                                         \
+    const unsigned g1 = (unsigned)((long)nseg * csam_cdiv(M, ROWS)), g4 = (unsigned)((long)nseg * csam_cdiv(M, 4 * ROWS)); \
+    const bool past = (long)M * ldy * sizeof(T) > (32L << 20) && aligned(y, ldy * sizeof(T), 128);                      \
+    if (past) mx_dequantize_kernel<T, F, 4, true><<<g4, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
+    else if (grid >= 2048) mx_dequantize_kernel<T, F, 4, false><<<g4, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
+    else mx_dequantize_kernel<T, F, 1, false><<<g1, 256, 0, st>>>((const uint8_t*)codes, ldcodes, (const uint8_t*)scales, scale_stride, (T*)y, ldy, M, K, nseg); \
   } while (0)
   if (fmt == CSAM_MX_FP4) {
     if (y_dtype == CSAM_DT_F16) GO(half_t, CSAM_MX_FP4);

@@ -1329,6 +1329,8 @@ def mx_gemm(a, w, out=None, bias=None, act=ACT_NONE, residual=None, out_dtype=to
         raise ValueError(f"{who}: activation {act!r}")
     M, lda, ass, ap, asp = _mx_check(a, who, "a")
     N, ldw, wss, wp, wsp = _mx_check(w, who, "w")
+    if lda >> 24 or ldw >> 24:
+        raise ValueError(f"{who}: code rows {max(lda, ldw)} bytes apart (less than 2^24)")
     ldr, r_dt, rp, bp = 0, 0, None, None
     if residual is not None:
         ldr, r_dt, rp = _mat(residual, who, "residual", M, N), _DT3[residual.dtype], residual.data_ptr()
@@ -1436,8 +1438,8 @@ def rotary(q, k, pos, freq, axis, interleaved=False, q_out=None, k_out=None):
     call on the output's gradient with ``-pos``."""
     who = "rotary"
     shape, dt = q.shape, q.dtype
-    if len(shape) != 3 or shape[0] > _INT_MAX or shape[2] == 0:
-        raise ValueError(f"{who}: q has shape {tuple(shape)}: {len(shape)} dimensions, not [tokens, heads, head_dim]")
+    if len(shape) != 3 or shape[0] > _INT_MAX or not 0 < shape[2] <= 4096:
+        raise ValueError(f"{who}: q has shape {tuple(shape)}: {len(shape)} dimensions, not [tokens, heads, head_dim <= 4096]")
     if dt not in _DT3:
         raise ValueError(f"{who}: q is {dt}, not float16, bfloat16 or float32")
     T, _, hd = shape

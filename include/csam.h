@@ -112,6 +112,7 @@ int csam_linear_f32_batched(void* stream, const float* A, long lda, long strideA
  *           16-byte aligned, ldcodes a multiple of 16;
  *   scales  E8M0 bytes, 2^(s - 127), 255 = NaN: block b = columns 32b .. 32b+31 of row r at scales[(b / 4) * scale_stride + r * 4 + b % 4];
  *           4-byte aligned, scale_stride a multiple of 4 and >= 4 * R.
+ * R and K are at most 2^31 - 256.
  * f16 / f32 / bf16 = CSAM_DT_F16 / _F32 / _BF16 in these entries and csam_rotary only. */
 #define CSAM_DT_BF16 2
 #define CSAM_MX_FP4 0
@@ -124,7 +125,8 @@ int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* c
 int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void* scales, long scale_stride, int fmt, void* y, long ldy,
                        int y_dtype, int M, int K);
 /* C[M,N] = act(A W^T + bias[n]) + residual[m,n]; A in either format, W in CSAM_MX_FP4, fp32 sums, one rounding to c_dtype.  bias
- * (fp32 [N]) and residual (f16 / f32 / bf16) may be NULL; C may be the residual itself.  K is the unpadded width; any M, N. */
+ * (fp32 [N]) and residual (f16 / f32 / bf16) may be NULL; C may be the residual itself.  K is the unpadded width, at most 2^20; code rows
+ * less than 2^24 bytes apart. */
 int csam_mx_gemm(void* stream, const void* A, long lda, const void* A_scales, long a_scale_stride, int a_fmt, const void* W, long ldw,
                  const void* W_scales, long w_scale_stride, void* C, long ldc, int c_dtype, const float* bias, const void* residual,
                  long ldr, int r_dtype, int act, int M, int N, int K);
@@ -139,7 +141,7 @@ int csam_rms_norm_mx(void* stream, const void* x, long ldx, int x_dtype, const v
  * radians, (a, b) -> (a cos - b sin, a sin + b cos).  Pairs are elements (p, p + pairs), or (2p, 2p + 1) if interleaved; elements from
  * 2 * pairs on are copied.  q [T][Hq][head_dim] with row pitch ldq and head pitch hsq in elements (k alike); the outputs may be the
  * inputs.  pos int32 or fp32 [axes][pos_stride], T a multiple of T_pos; freq fp64 [pairs]; axis int32 [pairs], clamped to 0 .. axes-1.
- * Angles are formed and reduced in fp64.  The adjoint is the call with negated positions. */
+ * Angles are formed and reduced in fp64.  head_dim <= 4096.  The adjoint is the call with negated positions. */
 int csam_rotary(void* stream, const void* q, long ldq, int hsq, void* q_out, long ldqo, int hsqo, int Hq, const void* k, long ldk, int hsk,
                 void* k_out, long ldko, int hsko, int Hk, int dtype, const void* pos, long pos_stride, int pos_is_f32, const double* freq,
                 const int* axis, int axes, int pairs, int interleaved, int T, int T_pos, int head_dim);

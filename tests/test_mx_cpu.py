@@ -53,6 +53,7 @@ def test_reference_rounds_ties_to_even_and_saturates():
     (lambda: hip.mx_gemm(mx(4, 256, "fp8"), mx(8, 256, "fp4"), residual=torch.zeros(8, 4)), "residual"),
     (lambda: hip.mx_gemm(mx(4, 256, "fp8"), mx(8, 256, "fp4"), out=torch.zeros(4, 9)), "out has shape"),
     (lambda: hip.mx_gemm(mx(4, 256, "fp8"), mx(8, 256, "fp4"), act=7), "activation"),
+    (lambda: hip.mx_gemm(hip.MxTensor(torch.empty(2, 1 << 24, dtype=torch.uint8)[:, :256], *mx(2, 256, "fp8")[1:]), mx(8, 256, "fp4")), "2\\^24"),
     (lambda: hip.mx_gemm(mx(4, 256, "fp8"), mx(8, 256, "fp4"), out_dtype=torch.float64), "float64"),
     (lambda: hip.mx_gemm(mx(4, 256, "fp8"), mx(8, 256, "fp4")), "no CPU form"),
     (lambda: hip.rms_norm(torch.zeros(4, 64), torch.zeros(64), 0.0), "eps"),
@@ -83,6 +84,7 @@ def rot(q=None, k=None, pos=None, pairs=8, axes=2, **kw):
     (lambda: rot(q=torch.zeros(6, 64)), "dimensions"),
     (lambda: rot(q=torch.zeros(6, 2, 32, dtype=torch.float64)), "float64"),
     (lambda: rot(pairs=17), "17 pairs"),
+    (lambda: rot(q=torch.zeros(6, 1, 4098)), "4096"),
     (lambda: rot(pos=torch.zeros(2, 4)), "multiple"),
     (lambda: rot(pos=torch.zeros(2, 6, dtype=torch.int64)), "pos"),
     (lambda: rot(pos=torch.zeros(6, 2).t()), "positions of an axis"),
