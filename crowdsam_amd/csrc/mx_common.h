@@ -32,41 +32,38 @@ __device__ __forceinline__ void csam_put(P* p, V v) {
   if constexpr (NT) __builtin_nontemporal_store(v, p);
   else *p = v;
 }
-// 8 consecutive elements as fp32; _tail: the first n of them (n may be <= 0), zeros behind
-template <typename T>
-__device__ __forceinline__ void csam_load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const auto a = *(const typename csam_pack<T, 4>::at*)p, b = *(const typename csam_pack<T, 4>::at*)(p + 4);
+// V = 4 or 8 consecutive elements as fp32; _tail: the first n of them (n may be <= 0), zeros behind
+template <typename T, int V>
+__device__ __forceinline__ void csam_load(const T* p, float (&v)[V]) {
+  constexpr int N = sizeof(T) == 4 ? 4 : V;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-  } else {
-    const auto h = *(const typename csam_pack<T, 8>::at*)p;
+  for (int j = 0; j < V; j += N) {
+    const auto h = *(const typename csam_pack<T, N>::at*)(p + j);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+    for (int i = 0; i < N; ++i) v[j + i] = (float)h[i];
   }
 }
-template <typename T>
-__device__ __forceinline__ void csam_load8_tail(const T* p, int n, float (&v)[8]) {
+template <typename T, int V>
+__device__ __forceinline__ void csam_load_tail(const T* p, int n, float (&v)[V]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+  for (int i = 0; i < V; ++i) v[i] = i < n ? (float)p[i] : 0.f;
 }
-// 8 consecutive elements, rounded to nearest even
-template <bool NT = false, typename T>
-__device__ __forceinline__ void csam_store8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    csam_put<NT>((typename csam_pack<T, 4>::at*)p, floatx4{v[0], v[1], v[2], v[3]});
-    csam_put<NT>((typename csam_pack<T, 4>::at*)(p + 4), floatx4{v[4], v[5], v[6], v[7]});
-  } else {
-    typename csam_pack<T, 8>::vec h;
+// V consecutive elements, rounded to nearest even
+template <bool NT = false, typename T, int V>
+__device__ __forceinline__ void csam_store(T* p, const float (&v)[V]) {
+  constexpr int N = sizeof(T) == 4 ? 4 : V;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (T)v[i];
-    csam_put<NT>((typename csam_pack<T, 8>::at*)p, h);
+  for (int j = 0; j < V; j += N) {
+    typename csam_pack<T, N>::vec h;
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = (T)v[j + i];
+    csam_put<NT>((typename csam_pack<T, N>::at*)(p + j), h);
   }
 }
-template <typename T>
-__device__ __forceinline__ void csam_store8_tail(T* p, int n, const float (&v)[8]) {
+template <typename T, int V>
+__device__ __forceinline__ void csam_store_tail(T* p, int n, const float (&v)[V]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < V; ++i)
     if (i < n) p[i] = (T)v[i];
 }
 
@@ -76,65 +73,74 @@ __device__ __forceinline__ float csam_e8m0(unsigned s) {
   return __builtin_bit_cast(float, bits);
 }
 
-// value of lane ^ 1 / ^ 2 within a quad, and the lane 4 / 8 further round within 16
+// DPP: a value of another lane of the quad, the eight or the row of sixteen
 template <int CTRL>
 __device__ __forceinline__ unsigned csam_dpp(unsigned v) {
   return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
 }
 
-// Quantises the 8 values of this lane, whose quad of lanes holds one block of 32: returns the block's E8M0 byte and the codes
-// (E2M1: 32 bits in c[0]; E4M3: 64 bits).
+// Quantises the V = 8 (4) values of this lane, whose quad (eight) of lanes holds one block of 32: returns the block's E8M0 byte and the
+// codes (E2M1: 4 V bits in c[0]; E4M3: 8 V bits).
 //   byte = max(exponent(amax) - emax, 0) on the biased fp32 exponent = floor(log2 amax) - emax + 127; a subnormal or zero amax has
 //   exponent field 0, so its byte is 0; NaN and infinity have 255 -> byte 255 (every value of the block reads as NaN), codes 0.
 // amax is an integer maximum of the magnitudes' bits: fmaxf would drop a NaN.  x / 2^(byte-127) is exact in fp32 (a power of two; the
 // only results that could be subnormal come from elements 2^-100 below the block's largest, which round to zero in either format),
 // so the one rounding is the converter's to E2M1 / E4M3, ties to even; both saturate (E4M3 by the clamp: the converter's own overflow
 // would give NaN).
-template <int FMT>
-__device__ __forceinline__ unsigned csam_mx_quant8(const float (&v)[8], unsigned (&c)[2]) {
+template <int FMT, int V>
+__device__ __forceinline__ unsigned csam_mx_quant(const float (&v)[V], unsigned (&c)[2]) {
   unsigned m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu);
+  for (int i = 0; i < V; ++i) m = max(m, __builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu);
   m = max(m, csam_dpp<0xB1>(m));                          // quad_perm 1,0,3,2
   m = max(m, csam_dpp<0x4E>(m));                          // quad_perm 2,3,0,1
+  if constexpr (V == 4) m = max(m, csam_dpp<0x141>(m));   // row_half_mirror: the other quad of the eight
   const unsigned e = m >> 23;
   constexpr unsigned EMAX = FMT == CSAM_MX_FP4 ? 2 : 8;
   const unsigned byte = e == 255u ? 255u : e > EMAX ? e - EMAX : 0u;
+  c[0] = c[1] = 0u;
   if constexpr (FMT == CSAM_MX_FP4) {
     const float scale = __builtin_bit_cast(float, byte == 0u ? 0x00400000u : byte << 23);
     unsigned q = 0;
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], scale, 0);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], scale, 1);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[4], v[5], scale, 2);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
+    if constexpr (V == 8) {
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[4], v[5], scale, 2);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
+    }
     c[0] = e == 255u ? 0u : q;
-    c[1] = 0u;
   } else {
     const float inv = __builtin_bit_cast(float, (254u - (byte > 253u ? 253u : byte)) << 23);
-    float w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -448.f, 448.f);
-    int a = 0, b = 0;
-    a = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], a, false);
-    a = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], a, true);
-    b = __builtin_amdgcn_cvt_pk_fp8_f32(w[4], w[5], b, false);
-    b = __builtin_amdgcn_cvt_pk_fp8_f32(w[6], w[7], b, true);
-    c[0] = e == 255u ? 0u : (unsigned)a;
-    c[1] = e == 255u ? 0u : (unsigned)b;
+    for (int j = 0; j < V / 4; ++j) {
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_fmed3f(v[4 * j + i] * inv, -448.f, 448.f);
+      int a = 0;
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], a, false);
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], a, true);
+      c[j] = e == 255u ? 0u : (unsigned)a;
+    }
   }
   return byte;
 }
 
-// Codes and scales of chunk `c8` (8 elements) of row `row`; 16 consecutive lanes hold a 128-wide group, so the four block bytes are
-// put together with two rotations within 16 lanes and leave as one dword.
-template <int FMT, bool NT = false>
-__device__ __forceinline__ void csam_mx_store8(const float (&v)[8], uint8_t* codes, long ldc, uint8_t* scales, long sstride, long row,
-                                               int c8) {
-  unsigned c[2];
-  unsigned s = csam_mx_quant8<FMT>(v, c) << (8 * ((c8 >> 2) & 3));
-  s |= csam_dpp<0x124>(s);                                // row_ror:4
-  s |= csam_dpp<0x128>(s);                                // row_ror:8
-  if constexpr (FMT == CSAM_MX_FP4) csam_put<NT>((unsigned*)(codes + row * ldc + c8 * 4), c[0]);
-  else csam_put<NT>((uintx2*)(codes + row * ldc + c8 * 8), uintx2{c[0], c[1]});
-  if ((c8 & 15) == 0) *(unsigned*)(scales + (long)(c8 >> 4) * sstride + row * 4) = s;
+// Codes and scales of chunk `c` (V elements) of row `row`.  V = 8: 16 consecutive lanes hold a 128-wide group, so the four block bytes are
+// put together with two rotations within 16 lanes and leave as one dword; V = 4: they are 32 lanes, and each block's byte leaves by itself.
+template <int FMT, bool NT = false, int V>
+__device__ __forceinline__ void csam_mx_store(const float (&v)[V], uint8_t* codes, long ldc, uint8_t* scales, long sstride, long row, int c) {
+  unsigned q[2];
+  unsigned s = csam_mx_quant<FMT>(v, q);
+  uint8_t* to = codes + row * ldc + c * (FMT == CSAM_MX_FP4 ? V / 2 : V);
+  if constexpr (FMT == CSAM_MX_FP8 && V == 8) csam_put<NT>((uintx2*)to, uintx2{q[0], q[1]});
+  else if constexpr (FMT == CSAM_MX_FP8 || V == 8) csam_put<NT>((unsigned*)to, q[0]);
+  else csam_put<NT>((unsigned short*)to, (unsigned short)q[0]);
+  if constexpr (V == 8) {
+    s <<= 8 * ((c >> 2) & 3);
+    s |= csam_dpp<0x124>(s);                              // row_ror:4
+    s |= csam_dpp<0x128>(s);                              // row_ror:8
+    if ((c & 15) == 0) *(unsigned*)(scales + (long)(c >> 4) * sstride + row * 4) = s;
+  } else {
+    if ((c & 7) == 0) scales[(long)(c >> 5) * sstride + row * 4 + ((c >> 3) & 3)] = (uint8_t)s;
+  }
 }

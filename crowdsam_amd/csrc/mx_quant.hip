@@ -25,14 +25,14 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
     if (row < M && k < K) {
-      if (k + 8 <= K) csam_load8(x + (long)row * ldx + k, v[i]);
-      else csam_load8_tail(x + (long)row * ldx + k, K - k, v[i]);
+      if (k + 8 <= K) csam_load(x + (long)row * ldx + k, v[i]);
+      else csam_load_tail(x + (long)row * ldx + k, K - k, v[i]);
     }
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = r0 + 8 * i;
-    if (row < M) csam_mx_store8<FMT, NT>(v[i], codes, ldc, scales, sstride, row, c8);       // whole half-waves share a row
+    if (row < M) csam_mx_store<FMT, NT>(v[i], codes, ldc, scales, sstride, row, c8);       // whole half-waves share a row
   }
 }
 
@@ -109,105 +109,136 @@ struct RmsArgs {
   float eps;
   void* y; long ldy; int y_kind;          // CSAM_DT_*, or RMS_MX + CSAM_MX_*
   uint8_t* scales; long sstride;
-  int M, D, Dp, rows;                     // rows: rows of a row slot (a wave when NW = 1, the workgroup otherwise)
+  int M, D, Dp;
 };
 constexpr int RMS_MX = 16;
-
-// RK: 0 no residual, 1 residual of x's type, 2 fp32 residual
-template <typename T, int RK, int NW, int MAXC>
+// RK: 0 no residual, 1 residual of x's type, 2 fp32 residual.  A lane's chunks are V elements: 8, or 4 where a stream of a row is fp32, so
+// that every access of a wave is one run (the two 16-byte halves of a lane's 8 fp32 values would part it: 65536 x 512 with an
+// fp32 residual 85 us, 68 so, and with all of a row's loads in flight).
+template <typename T, int RK, int NW, int MAXC, int V, bool NT>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsArgs p) {
   typedef typename std::conditional<RK == 2, float, T>::type R;
   constexpr int SLOTS = NW == 1 ? 4 : 1;
-  __shared__ float part[2][NW];
+  __shared__ float part[NW];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int slot = NW == 1 ? wave : 0;
   const int c0 = NW == 1 ? lane : (int)threadIdx.x;
   constexpr int STEP = NW * 64;
+  const long row = (long)blockIdx.x * SLOTS + slot;
+  if (row >= p.M) return;                                  // uniform over the waves that share the row
   const int D = p.D;
-  float g[MAXC][8];
-#pragma unroll
-  for (int j = 0; j < MAXC; ++j) {
-    const int k = (c0 + j * STEP) * 8;
-    if (k + 8 <= D) csam_load8(p.gamma + k, g[j]);
-    else csam_load8_tail(p.gamma + k, D - k, g[j]);
-  }
-  const float inv_d = 1.0f / (float)D;
-  for (int i = 0; i < p.rows; ++i) {
-    const long row = (long)blockIdx.x * SLOTS * p.rows + (long)i * SLOTS + slot;
-    if (row >= p.M) break;                                 // uniform over the waves that share the row
-    float v[MAXC][8];
-    float s = 0.f;
+  const T* xr = (const T*)p.x + row * p.ldx;
+  const R* rr = (const R*)p.r + row * p.ldr;
+  // Where a whole chunk begins; lanes without one load the row's first and drop it, so that no branch parts the loads and all of a row's
+  // are in flight at once (65536 x 1280 fp16 with an fp32 residual to E4M3: 202 us with a branch at every chunk, 169 so).
+  auto at = [&](int j) {
+    const int k = (c0 + j * STEP) * V;
+    return k + V <= D ? k : 0;
+  };
+  float v[MAXC][V], g[MAXC][V];
+  float s = 0.f;
+  if (D >= V) {
+    typename csam_pack<T, V>::vec x[MAXC];
+    typename csam_pack<R, V>::vec r[MAXC];
 #pragma unroll
     for (int j = 0; j < MAXC; ++j) {
-      const int k = (c0 + j * STEP) * 8;
+      x[j] = *(const typename csam_pack<T, V>::at*)(xr + at(j));
+      if constexpr (RK != 0) r[j] = *(const typename csam_pack<R, V>::at*)(rr + at(j));
+    }
+    if constexpr (NW < 16) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-      if (k < D) {
-        const bool full = k + 8 <= D;
-        const T* xp = (const T*)p.x + row * p.ldx + k;
-        if (full) csam_load8(xp, v[j]);
-        else csam_load8_tail(xp, D - k, v[j]);
-        if constexpr (RK != 0) {
-          float r[8];
-          const R* rp = (const R*)p.r + row * p.ldr + k;
-          if (full) csam_load8(rp, r);
-          else csam_load8_tail(rp, D - k, r);
+      for (int j = 0; j < MAXC; ++j) csam_load(p.gamma + at(j), g[j]);
+    }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[j][e] += r[e];
-          R* hp = (R*)p.h + row * p.ldh + k;
-          if (full) csam_store8(hp, v[j]);
-          else csam_store8_tail(hp, D - k, v[j]);
-        }
+    for (int j = 0; j < MAXC; ++j) {
+      const bool full = (c0 + j * STEP) * V + V <= D;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(v[j][e], v[j][e], s);
+      for (int e = 0; e < V; ++e) {
+        float h = (float)x[j][e];
+        if constexpr (RK != 0) h += (float)r[j][e];
+        v[j][e] = full ? h : 0.f;
+        if constexpr (NW < 16) g[j][e] = full ? g[j][e] : 0.f;     // (columns behind D are zero, whatever gamma holds)
       }
     }
-    s = csam_wave_sum(s);
-    if constexpr (NW > 1) {
-      if (lane == 0) part[i & 1][wave] = s;                // two buffers: a row's partials are read after the barrier that its
-      __syncthreads();                                     // writes precede, and overwritten after the next row's barrier
-      s = 0.f;
+  } else {
 #pragma unroll
-      for (int w = 0; w < NW; ++w) s += part[i & 1][w];
-    }
-    const float rstd = 1.0f / sqrtf(s * inv_d + p.eps);
+    for (int j = 0; j < MAXC; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[j][e] = g[j][e] = 0.f;
+  }
+  if (D % V != 0) {
 #pragma unroll
     for (int j = 0; j < MAXC; ++j) {
-      const int c = c0 + j * STEP, k = c * 8;
-      float y[8];
+      const int k = (c0 + j * STEP) * V;
+      if (k < D && k + V > D) {
+        csam_load_tail(xr + k, D - k, v[j]);
+        if constexpr (NW < 16) csam_load_tail(p.gamma + k, D - k, g[j]);
+        if constexpr (RK != 0) {
+          float r[V];
+          csam_load_tail(rr + k, D - k, r);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = v[j][e] * rstd * g[j][e];
-      if (p.y_kind >= RMS_MX) {
-        if (k < p.Dp) {                                    // whole groups of 32 lanes: Dp is a multiple of 256
-          if (p.y_kind == RMS_MX + CSAM_MX_FP8) csam_mx_store8<CSAM_MX_FP8>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
-          else csam_mx_store8<CSAM_MX_FP4>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
+          for (int e = 0; e < V; ++e) v[j][e] += r[e];
         }
-      } else if (k < D) {
-        const bool full = k + 8 <= D;
-        if (p.y_kind == CSAM_DT_F16) {
-          half_t* yp = (half_t*)p.y + row * p.ldy + k;
-          if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
-        } else if (p.y_kind == CSAM_DT_BF16) {
-          bf16_t* yp = (bf16_t*)p.y + row * p.ldy + k;
-          if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
-        } else {
-          float* yp = (float*)p.y + row * p.ldy + k;
-          if (full) csam_store8(yp, y); else csam_store8_tail(yp, D - k, y);
-        }
+      }
+    }
+  }
+  if constexpr (RK != 0) {
+#pragma unroll
+    for (int j = 0; j < MAXC; ++j) {
+      const int k = (c0 + j * STEP) * V;
+      R* hp = (R*)p.h + row * p.ldh + k;
+      if (k + V <= D) csam_store<NT>(hp, v[j]);
+      else csam_store_tail(hp, D - k, v[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MAXC; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) s = fmaf(v[j][e], v[j][e], s);
+  s = csam_wave_sum(s);
+  if constexpr (NW > 1) {
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) s += part[w];
+  }
+  const float rstd = 1.0f / sqrtf(s * (1.0f / (float)D) + p.eps);
+#pragma unroll
+  for (int j = 0; j < MAXC; ++j) {
+    const int c = c0 + j * STEP, k = c * V;
+    if constexpr (NW == 16) {                              // (fewer registers: 4000 x 32768 bfloat16 266 us with gamma held from the start, 204 so)
+      if (k + V <= D) csam_load(p.gamma + k, g[j]);
+      else csam_load_tail(p.gamma + k, D - k, g[j]);
+    }
+    float y[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = v[j][e] * rstd * g[j][e];
+    if (p.y_kind >= RMS_MX) {
+      if (k < p.Dp) {                                    // whole blocks of lanes: Dp is a multiple of 256
+        if (p.y_kind == RMS_MX + CSAM_MX_FP8) csam_mx_store<CSAM_MX_FP8, NT>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
+        else csam_mx_store<CSAM_MX_FP4, NT>(y, (uint8_t*)p.y, p.ldy, p.scales, p.sstride, row, c);
+      }
+    } else if (k < D) {
+      const bool full = k + V <= D;
+      if (p.y_kind == CSAM_DT_F16) {
+        half_t* yp = (half_t*)p.y + row * p.ldy + k;
+        if (full) csam_store<NT>(yp, y); else csam_store_tail(yp, D - k, y);
+      } else if (p.y_kind == CSAM_DT_BF16) {
+        bf16_t* yp = (bf16_t*)p.y + row * p.ldy + k;
+        if (full) csam_store<NT>(yp, y); else csam_store_tail(yp, D - k, y);
+      } else {
+        float* yp = (float*)p.y + row * p.ldy + k;
+        if (full) csam_store<NT>(yp, y); else csam_store_tail(yp, D - k, y);
       }
     }
   }
 }
 
-template <typename T, int RK>
-int rms_launch(hipStream_t st, RmsArgs& p) {
-  const int chunks = csam_cdiv(p.Dp ? p.Dp : p.D, 8);
-#define RMS_GO(NW, MAXC)                                                                              \
-  do {                                                                                                \
-    const int slots = NW == 1 ? 4 : 1;                                                                \
-    p.rows = max(1, min(16, p.M / (4096 / NW)));                                                      \
-    rms_norm_kernel<T, RK, NW, MAXC><<<csam_cdiv(p.M, (long)slots * p.rows), NW == 1 ? 256 : NW * 64, 0, st>>>(p); \
-  } while (0)
+template <typename T, int RK, int V, bool NT>
+int rms_launch_v(hipStream_t st, const RmsArgs& p) {
+  const int chunks = csam_cdiv(p.Dp ? p.Dp : p.D, 8);      // of 8
+#define RMS_GO(NW, MAXC) rms_norm_kernel<T, RK, NW, MAXC * 8 / V, V, NT><<<csam_cdiv(p.M, NW == 1 ? 4 : 1), NW == 1 ? 256 : NW * 64, 0, st>>>(p)
   if (chunks <= 64) RMS_GO(1, 1);
   else if (chunks <= 128) RMS_GO(1, 2);
   else if (chunks <= 192) RMS_GO(1, 3);
@@ -218,6 +249,18 @@ int rms_launch(hipStream_t st, RmsArgs& p) {
 #undef RMS_GO
   CSAM_LAUNCH_CHECK("csam_rms_norm");
   return CSAM_OK;
+}
+
+template <typename T, int RK>
+int rms_launch(hipStream_t st, const RmsArgs& p) {
+  const long yb = p.y_kind >= RMS_MX ? 1 : p.y_kind == CSAM_DT_F32 ? 4 : 2, hb = RK == 0 ? 0 : RK == 2 ? 4 : (long)sizeof(T);
+  // Results that the last-level cache would not hold go past the caches (65536 x 1280 bfloat16, 336 MB: 115 us, 113 so); smaller ones stay
+  // for their reader (21320 x 1024 fp16 with an fp32 residual to E4M3: 43 us, 39 past the caches, but with the product that reads both 83,
+  // past the caches 88).
+  const bool past = (long)p.M * p.D * (yb + hb) > (256L << 20);
+  if constexpr (sizeof(T) == 4 || RK == 2) return past ? rms_launch_v<T, RK, 4, true>(st, p) : rms_launch_v<T, RK, 4, false>(st, p);
+  else if (p.y_kind == CSAM_DT_F32) return past ? rms_launch_v<T, RK, 4, true>(st, p) : rms_launch_v<T, RK, 4, false>(st, p);
+  else return past ? rms_launch_v<T, RK, 8, true>(st, p) : rms_launch_v<T, RK, 8, false>(st, p);
 }
 
 bool aligned(const void* p, long ld_bytes, int a) { return ((uintptr_t)p % a) == 0 && ld_bytes % a == 0; }
@@ -326,7 +369,7 @@ int csam_rms_norm(void* stream, const void* x, long ldx, int x_dtype, const void
                   const float* gamma, float eps, void* y, long ldy, int y_dtype, int M, int D) {
   if (M == 0) return CSAM_OK;
   CSAM_REQUIRE(dt_ok(y_dtype) && ldy >= D, "csam_rms_norm: bad output dtype %d or row pitch %ld", y_dtype, ldy);
-  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0, 1};
+  RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, y, ldy, y_dtype, nullptr, 0, M, D, 0};
   return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm");
 }
 
@@ -336,7 +379,7 @@ int csam_rms_norm_mx(void* stream, const void* x, long ldx, int x_dtype, const v
   CSAM_REQUIRE(D > 0, "csam_rms_norm_mx: bad width %d", D);
   if (int rc = mx_check("csam_rms_norm_mx", codes, ldcodes, scales, scale_stride, fmt, M, D)) return rc;
   RmsArgs p = {x, ldx, residual, ldr, h, ldh, gamma, eps, codes, ldcodes, RMS_MX + fmt, (uint8_t*)scales, scale_stride, M, D,
-               csam_cdiv(D, 256) * 256, 1};
+               csam_cdiv(D, 256) * 256};
   return rms_any((hipStream_t)stream, p, x_dtype, r_dtype, "csam_rms_norm_mx");
 }
 
