@@ -7,8 +7,8 @@
 // differently: lane group g holds halves g (16 codes) of BOTH blocks.
 // What the instruction keeps: E2M1 products are summed as fp32 sums them.  With an E4M3 operand it lines 16 neighbouring products up to
 // the largest and drops bits below 2^-13 of that (measured: a product 2^-14 of its neighbour vanishes, one in the next 16 does not); on
-// gaussian rows the result is 4.5e-6 off in norm, against the 2e-2 that rounding the operand to E4M3 cost.  Taking the 16 apart would
-// double the instructions.
+// gaussian rows the result is 4.5e-6 off in norm, against the 2e-2 that rounding the operand to E4M3 cost.  16-bit results take that; fp32
+// results only where the caller says so, otherwise both operands are multiplied as bf16, which holds them exactly.
 // W rows are the instruction's row operand, A rows its columns: a lane ends up with 4 consecutive n of one row m.
 #include <type_traits>
 #include <utility>
@@ -24,6 +24,7 @@ struct MxGemmArgs {
   const float* bias;
   const void* R; long ldr; int r_dt;
   int act, M, N, Kp;
+  int cut;                                   // fp32 results may lose what the scaled instruction drops
   int past;                                  // C's rows begin on lines of 128 bytes: large tiles may store past the caches
 };
 
@@ -193,6 +194,58 @@ __device__ __forceinline__ intx8 mx_frag(const void* lo, const void* hi) {
   return intx8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
 }
 
+// An E4M3 part whose products are summed as fp32 sums them: both operands become bf16, which holds a scaled code of either format exactly,
+// and four 32x32x16 instructions take the part.  Lane group g then holds codes 16g .. 16g + 15 of both blocks of the part: A's fragment is
+// that already, W's group has 32 codes of one block and swaps halves with the other group, as the two groups' scales do.
+__device__ __forceinline__ void mx_swap32(unsigned& a, unsigned& b) {          // a's upper half of lanes for b's lower
+  const auto p = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = p[0];
+  b = p[1];
+}
+typedef __bf16 mx_bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx_bf8 __attribute__((ext_vector_type(8)));
+template <int KK>
+__device__ __forceinline__ void mx_scales(int s, unsigned (&byte)[2]) {        // of the part's two blocks
+  byte[0] = byte[1] = (unsigned)s;
+  mx_swap32(byte[0], byte[1]);
+#pragma unroll
+  for (int f = 0; f < 2; ++f) byte[f] = (byte[f] >> (8 * KK)) & 255u;
+}
+// a NaN block, or codes whose scale is so near the ends of the range that their product with it may not be a normal bf16
+__device__ __forceinline__ bool mx_far(unsigned byte, unsigned codes) { return byte == 255u || (byte - 32u >= 192u && codes != 0u); }
+template <int KK>
+__device__ __forceinline__ bool mx_bf16_a(const intx8& f, int s, mx_bf8 (&out)[4]) {
+  unsigned byte[2];
+  mx_scales<KK>(s, byte);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const float sc = __builtin_bit_cast(float, byte[m / 2] << 23);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const mx_bf2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * m + d], sc, false);
+      const mx_bf2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * m + d], sc, true);
+      out[m][4 * d] = lo[0], out[m][4 * d + 1] = lo[1], out[m][4 * d + 2] = hi[0], out[m][4 * d + 3] = hi[1];
+    }
+  }
+  return mx_far(byte[0], (unsigned)(f[0] | f[1] | f[2] | f[3])) || mx_far(byte[1], (unsigned)(f[4] | f[5] | f[6] | f[7]));
+}
+template <int KK>
+__device__ __forceinline__ bool mx_bf16_w(const intx8& f, int s, mx_bf8 (&out)[4]) {
+  unsigned byte[2];
+  mx_scales<KK>(s, byte);
+  unsigned q[4] = {(unsigned)f[0], (unsigned)f[1], (unsigned)f[2], (unsigned)f[3]};      // the first 16 codes, the others
+  mx_swap32(q[0], q[2]);                                                                   // of the part's first block, of its second
+  mx_swap32(q[1], q[3]);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const float sc = __builtin_bit_cast(float, byte[m / 2] << 23);
+    const mx_bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 1);
+    const mx_bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 3);
+    out[m] = mx_bf8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+  return mx_far(byte[0], q[0] | q[1]) || mx_far(byte[1], q[2] | q[3]);
+}
+
 // --------------------------------------------------------------------------------------------------------------- tiled form
 // TM x TN tile, WGM x WGN waves of 32x32 MFMA tiles, KS-wide steps through NS LDS stages filled by LDS-DMA (codes 16 bytes, scales 4
 // bytes per lane).  LDS lines are 128 bytes: a row of the step (256 E2M1 or 128 E4M3 codes), or two rows of 128 E2M1 codes.  The LDS reads
@@ -236,7 +289,7 @@ template <int N, typename F>
 __device__ __forceinline__ void mx_for(F f) { mx_for_each(std::make_integer_sequence<int, N>{}, f); }
 #define MX_C(x) (std::integral_constant<int, (x)>{})
 
-template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS>
+template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS, bool EXACT = false>
 __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 ? 1 : 2) void mx_gemm_kernel(MxGemmArgs p) {
   using T = MxTile<FA, TM, TN, WGM, WGN, NS, KS>;
   constexpr int NW = T::NW, RA = T::RA, RW = T::RW, LA = T::LA, LW = T::LW, LS = T::LS, MI = T::MI, NI = T::NI, NH = KS / 64;
@@ -330,10 +383,24 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
     constexpr int h = decltype(h_)::value, ss = decltype(ss_)::value, rh = decltype(rh_)::value;
     constexpr int d0 = decltype(d0_)::value, d1 = decltype(d1_)::value;
     constexpr int S = (rh & 1) == 0 ? NSC : 0, NR = NF + S, ND = d1 - d0;
+    mx_bf8 ab[EXACT ? MI : 1][4], wb[EXACT ? NI : 1][4];
+    bool far = false;
+    if constexpr (EXACT) {                                // (parts with scales at the ends of the range take the scaled instruction)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) far |= mx_bf16_a<(h & 1)>(af[h & 1][i], sa[ss][i], ab[i]);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) far |= mx_bf16_w<(h & 1)>(wf[h & 1][j], sw[ss][j], wb[j]);
+      far = __any(far);
+    }
     constexpr int GAPS = NQ < 4 ? NQ : 4, RPG = (NR + GAPS - 1) / GAPS, G0 = NQ > 4 ? 2 : 0;
     mx_for<NQ>([&](auto q_) {
       constexpr int q = decltype(q_)::value, i = q / NI, j = q % NI;
-      acc[i][j] = mx_mfma32<FA, (h & 1)>(wf[h & 1][j], af[h & 1][i], acc[i][j], sw[ss][j], sa[ss][i]);
+      if (EXACT && !far) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[EXACT ? j : 0][m], ab[EXACT ? i : 0][m], acc[i][j], 0, 0, 0);
+      } else {
+        acc[i][j] = mx_mfma32<FA, (h & 1)>(wf[h & 1][j], af[h & 1][i], acc[i][j], sw[ss][j], sa[ss][i]);
+      }
       __builtin_amdgcn_sched_barrier(0);
       constexpr int r0 = q * RPG < NR ? q * RPG : NR, r1 = (q + 1) * RPG < NR ? (q + 1) * RPG : NR;
       constexpr int e0 = q < G0 ? 0 : (q - G0) * ND / (NQ - G0), e1 = q < G0 ? 0 : (q - G0 + 1) * ND / (NQ - G0);
@@ -469,11 +536,11 @@ __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(MxGemmArgs p) {
   }
 }
 
-template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS>
+template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS, bool EXACT = false>
 int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
   const long grid = (long)csam_cdiv(p.M, TM) * csam_cdiv(p.N, TN);
   CSAM_REQUIRE(grid < (1L << 31), "csam_mx_gemm: too many tiles");
-  mx_gemm_kernel<FA, TM, TN, WGM, WGN, NS, KS><<<(unsigned)grid, WGM * WGN * 64, 0, st>>>(p);
+  mx_gemm_kernel<FA, TM, TN, WGM, WGN, NS, KS, EXACT><<<(unsigned)grid, WGM * WGN * 64, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_mx_gemm");
   return CSAM_OK;
 }
@@ -496,6 +563,15 @@ int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
 //   16384 x 4096 x 4096    128x128 218, 256x256 183                   128x256 292, 256x256 267
 template <int FA>
 int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
+  if constexpr (FA == CSAM_MX_FP8) {
+    // fp32 results keep what the scaled instruction drops, unless the caller lets it go.  us to fp32 (M x N x K), as bf16 / scaled to
+    // fp16, the conversion to bf16 taking most of the difference: 224 x 2048 x 1024 10.7 / 4.8, 5330 x 4096 x 1024 84 / 32;
+    // error in norm 7e-9 / 4.5e-6 before the rounding.
+    if (p.c_dt == CSAM_DT_F32 && !p.cut) {
+      if ((long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128) >= 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 128, true>(st, p);
+      return mx_tiles<FA, 64, 64, 2, 2, 4, 128, true>(st, p);
+    }
+  }
   const long t16 = (long)csam_cdiv(p.M, 16) * csam_cdiv(p.N, 16);
   if (p.M <= 16 || t16 <= 512) {
     if (t16 <= 256 || p.M <= 16) mx_gemm_rows_kernel<FA, 1, 4><<<(unsigned)t16, 256, 0, st>>>(p);
@@ -540,7 +616,8 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
   auto dt_ok = [](int dt) { return dt == CSAM_DT_F16 || dt == CSAM_DT_F32 || dt == CSAM_DT_BF16; };
   auto al = [](const void* q, long ld, int a) { return (uintptr_t)q % a == 0 && ld % a == 0; };
   CSAM_REQUIRE(dt_ok(c_dtype) && (!residual || dt_ok(r_dtype)), "csam_mx_gemm: bad dtype");
-  CSAM_REQUIRE(act == CSAM_ACT_NONE || act == CSAM_ACT_GELU || act == CSAM_ACT_RELU, "csam_mx_gemm: bad activation %d", act);
+  const int plain = act & ~CSAM_MX_CUT;
+  CSAM_REQUIRE(plain == CSAM_ACT_NONE || plain == CSAM_ACT_GELU || plain == CSAM_ACT_RELU, "csam_mx_gemm: bad activation %d", act);
   CSAM_REQUIRE(lda >= (a_fmt == CSAM_MX_FP8 ? Kp : Kp / 2) && ldw >= Kp / 2, "csam_mx_gemm: code rows are shorter than %d padded columns", Kp);
   CSAM_REQUIRE(lda < (1 << 24) && ldw < (1 << 24), "csam_mx_gemm: code rows 16 MB apart or more");
   CSAM_REQUIRE(al(A, lda, 16) && al(W, ldw, 16), "csam_mx_gemm: codes and their row pitch have to be multiples of 16 bytes");
@@ -548,6 +625,6 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
                "csam_mx_gemm: scale groups have to lie 4-byte aligned, at least 4 * rows bytes apart");
   CSAM_REQUIRE(ldc >= N && (!residual || ldr >= N), "csam_mx_gemm: an output row pitch is shorter than N");
   MxGemmArgs p = {(const uint8_t*)A, lda, (const uint8_t*)A_scales, a_scale_stride, (const uint8_t*)W, ldw, (const uint8_t*)W_scales,
-                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act, M, N, Kp, al(C, ldc * (c_dtype == CSAM_DT_F32 ? 4 : 2), 128)};
+                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act & ~CSAM_MX_CUT, M, N, Kp, act & CSAM_MX_CUT, al(C, ldc * (c_dtype == CSAM_DT_F32 ? 4 : 2), 128)};
   return a_fmt == CSAM_MX_FP8 ? mx_gemm_launch<CSAM_MX_FP8>((hipStream_t)stream, p) : mx_gemm_launch<CSAM_MX_FP4>((hipStream_t)stream, p);
 }
