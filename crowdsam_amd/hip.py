@@ -1319,7 +1319,7 @@ def mx_gemm(a, w, out=None, bias=None, act=ACT_NONE, residual=None, out_dtype=to
     """out[M, N] = act(a w^T + bias) + residual of two ``MxTensor``s: ``a`` [M, K] in "fp4" or "fp8", ``w`` [N, K] in "fp4"; fp32 sums,
     rounded once to ``out``'s type or ``out_dtype``.  ``bias`` fp32 [N]; ``residual`` [M, N] fp16 / bfloat16 / fp32; ``out`` may be the residual.  The kernel and with it the
     order of the sum depend on the sizes: rows are not bitwise independent of M.  ``cut``: an fp32 result of an "fp8" ``a`` may lose bits
-    below 2^-13 of the largest of 16 neighbouring products, as 16-bit results always do (4.5e-6 of the result's norm); two to three times
+    below 2^-13 of the largest of 16 neighbouring products, as 16-bit results always do (4.5e-6 of the result's norm); two to four times
     faster."""
     who = "mx_gemm"
     if w.fmt != "fp4":

@@ -128,7 +128,7 @@ int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void
 /* C[M,N] = act(A W^T + bias[n]) + residual[m,n]; A in either format, W in CSAM_MX_FP4, fp32 sums, one rounding to c_dtype.  bias
  * (fp32 [N]) and residual (f16 / f32 / bf16) may be NULL; C may be the residual itself.  An E4M3 A whose C is 16 bits wide is multiplied
  * by an instruction that drops bits below 2^-13 of the largest of 16 neighbouring products (4.5e-6 of the result's norm); for an fp32 C
- * nothing is dropped, at two to three times the time, unless act has CSAM_MX_CUT.  K is the unpadded width, at most 2^20; code rows
+ * nothing is dropped, at two to four times the time, unless act has CSAM_MX_CUT.  K is the unpadded width, at most 2^20; code rows
  * less than 2^24 bytes apart. */
 int csam_mx_gemm(void* stream, const void* A, long lda, const void* A_scales, long a_scale_stride, int a_fmt, const void* W, long ldw,
                  const void* W_scales, long w_scale_stride, void* C, long ldc, int c_dtype, const float* bias, const void* residual,
