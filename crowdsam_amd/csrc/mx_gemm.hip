@@ -212,7 +212,7 @@ __device__ __forceinline__ void mx_scales(int s, unsigned (&byte)[2]) {        /
   for (int f = 0; f < 2; ++f) byte[f] = (byte[f] >> (8 * KK)) & 255u;
 }
 // a NaN block, or codes whose scale is so near the ends of the range that their product with it may not be a normal bf16
-__device__ __forceinline__ bool mx_far(unsigned byte, unsigned codes) { return byte == 255u || (byte - 32u >= 192u && codes != 0u); }
+__device__ __forceinline__ bool mx_far(unsigned byte, unsigned codes) { return (byte == 255u) | ((byte - 32u >= 192u) & (codes != 0u)); }
 template <int KK>
 __device__ __forceinline__ bool mx_bf16_a(const intx8& f, int s, mx_bf8 (&out)[4]) {
   unsigned byte[2];
@@ -227,7 +227,7 @@ __device__ __forceinline__ bool mx_bf16_a(const intx8& f, int s, mx_bf8 (&out)[4
       out[m][4 * d] = lo[0], out[m][4 * d + 1] = lo[1], out[m][4 * d + 2] = hi[0], out[m][4 * d + 3] = hi[1];
     }
   }
-  return mx_far(byte[0], (unsigned)(f[0] | f[1] | f[2] | f[3])) || mx_far(byte[1], (unsigned)(f[4] | f[5] | f[6] | f[7]));
+  return mx_far(byte[0], (unsigned)(f[0] | f[1] | f[2] | f[3])) | mx_far(byte[1], (unsigned)(f[4] | f[5] | f[6] | f[7]));
 }
 template <int KK>
 __device__ __forceinline__ bool mx_bf16_w(const intx8& f, int s, mx_bf8 (&out)[4]) {
@@ -243,7 +243,7 @@ __device__ __forceinline__ bool mx_bf16_w(const intx8& f, int s, mx_bf8 (&out)[4
     const mx_bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 3);
     out[m] = mx_bf8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   }
-  return mx_far(byte[0], q[0] | q[1]) || mx_far(byte[1], q[2] | q[3]);
+  return mx_far(byte[0], q[0] | q[1]) | mx_far(byte[1], q[2] | q[3]);
 }
 
 // --------------------------------------------------------------------------------------------------------------- tiled form
@@ -391,28 +391,32 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
       for (int i = 0; i < MI; ++i) far |= mx_bf16_a<(h & 1)>(af[h & 1][i], sa[ss][i], ab[i]);
 #pragma unroll
       for (int j = 0; j < NI; ++j) far |= mx_bf16_w<(h & 1)>(wf[h & 1][j], sw[ss][j], wb[j]);
-      far = __any(far);
+      far = __builtin_amdgcn_ballot_w64(far) != 0;        // uniform: matrix instructions do not heed the lanes' mask
     }
     constexpr int GAPS = NQ < 4 ? NQ : 4, RPG = (NR + GAPS - 1) / GAPS, G0 = NQ > 4 ? 2 : 0;
-    mx_for<NQ>([&](auto q_) {
-      constexpr int q = decltype(q_)::value, i = q / NI, j = q % NI;
-      if (EXACT && !far) {
+    auto run = [&](auto bf_) {
+      mx_for<NQ>([&](auto q_) {
+        constexpr int q = decltype(q_)::value, i = q / NI, j = q % NI;
+        if constexpr (decltype(bf_)::value) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[EXACT ? j : 0][m], ab[EXACT ? i : 0][m], acc[i][j], 0, 0, 0);
-      } else {
-        acc[i][j] = mx_mfma32<FA, (h & 1)>(wf[h & 1][j], af[h & 1][i], acc[i][j], sw[ss][j], sa[ss][i]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      constexpr int r0 = q * RPG < NR ? q * RPG : NR, r1 = (q + 1) * RPG < NR ? (q + 1) * RPG : NR;
-      constexpr int e0 = q < G0 ? 0 : (q - G0) * ND / (NQ - G0), e1 = q < G0 ? 0 : (q - G0 + 1) * ND / (NQ - G0);
-      mx_for<r1 - r0>([&](auto x_) {
-        constexpr int k = r0 + decltype(x_)::value;
-        if constexpr (k < S) read_scale(MX_C(k), rh_, rs_, rslot);
-        else read(MX_C(k - S), rh_, rslot);
+          for (int m = 0; m < 4; ++m) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j][m], ab[i][m], acc[i][j], 0, 0, 0);
+        } else {
+          acc[i][j] = mx_mfma32<FA, (h & 1)>(wf[h & 1][j], af[h & 1][i], acc[i][j], sw[ss][j], sa[ss][i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int r0 = q * RPG < NR ? q * RPG : NR, r1 = (q + 1) * RPG < NR ? (q + 1) * RPG : NR;
+        constexpr int e0 = q < G0 ? 0 : (q - G0) * ND / (NQ - G0), e1 = q < G0 ? 0 : (q - G0 + 1) * ND / (NQ - G0);
+        mx_for<r1 - r0>([&](auto x_) {
+          constexpr int k = r0 + decltype(x_)::value;
+          if constexpr (k < S) read_scale(MX_C(k), rh_, rs_, rslot);
+          else read(MX_C(k - S), rh_, rslot);
+        });
+        mx_for<e1 - e0>([&](auto x_) { dma(MX_C(d0 + e0 + decltype(x_)::value), dslot, dt); });
+        __builtin_amdgcn_sched_barrier(0);
       });
-      mx_for<e1 - e0>([&](auto x_) { dma(MX_C(d0 + e0 + decltype(x_)::value), dslot, dt); });
-      __builtin_amdgcn_sched_barrier(0);
-    });
+    };
+    if (EXACT && !far) run(std::integral_constant<bool, EXACT>{});
+    else run(std::false_type{});
   };
   constexpr int FIRST = (PER + NH - 1) / NH;              // DMAs of a stage that its first (the last) part issues
   mx_for<NS - 1>([&](auto s_) { mx_for<PER>([&](auto d_) { dma(d_, decltype(s_)::value, min(decltype(s_)::value, nt - 1)); }); });
@@ -567,7 +571,7 @@ template <int FA>
 int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
   if constexpr (FA == CSAM_MX_FP8) {
     // fp32 results keep what the scaled instruction drops, unless the caller lets it go.  us to fp32 (M x N x K), as bf16 / scaled to
-    // fp16, the conversion to bf16 taking most of the difference: 224 x 2048 x 1024 10.7 / 4.8, 5330 x 4096 x 1024 86 / 32;
+    // fp16, the conversion to bf16 taking most of the difference: 224 x 2048 x 1024 9.4 / 4.9, 5330 x 4096 x 1024 75 / 34;
     // error in norm 7e-9 / 4.5e-6 before the rounding.
     if (p.c_dt == CSAM_DT_F32 && !p.cut) {
       if ((long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128) >= 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 128, true>(st, p);
