@@ -93,10 +93,11 @@ __device__ __forceinline__ float csam_gelu_erf(float x) {
   return 0.5f * x * (1.0f + csam_erf_fast(x * 0.70710678118654752440f));
 }
 // Packed-fp32 polynomial GELU for fp16-bound outputs (the fused upscaler, which PMC shows VALU-bound on GELU):
-//   Phi(x) ~ 0.5 + xc * R(xc^2),  xc = clamp(x, +-4.4),  R = degree-8 minimax fit with Phi(4.4) = 1 exactly,
-// |gelu error| <= 2.5e-5 for |x| < 3 and <= 6.5e-5 overall (at x = -4.35; 4.5e-5 on the grid of tools/fit_gelu_poly.py) -- an order below the fp16
-// rounding of the value it feeds -- in 13 instructions per PAIR (v_med3 x2, 11 v_pk_*_f32), no transcendental,
-// against ~22 issue slots per element for the erf form above.
+//   Phi(x) ~ 0.5 + xc * R(xc^2),  xc = clamp(x, +-4.4),  R = degree-8 minimax fit with Phi(4.4) = 1 (tools/fit_gelu_poly.py).
+// In fp32: |gelu error| <= 4.1e-5 for |x| < 3, <= 8.1e-5 up to the clamp (at x = -4.34; 4.5e-5 on the fit's grid), and 1.31e-6 |x|
+// beyond it, where Phi stays 1.0000013 or -1.3e-6.  That is below half an fp16 step of the result where the result is over 0.17; of the
+// small negative results it is many steps, and x far below -4.4 gives a small POSITIVE value.
+// 13 instructions per PAIR (v_med3 x2, 11 v_pk_*_f32), no transcendental, against ~22 issue slots per element for the erf form above.
 // (Round 5 tried the clamp on the OUTPUT instead -- the VOP3P `clamp` bit of the last packed FMA, which needs a one-instruction
 // inline asm because hipcc does not fold it: -7 % VALU instructions in the upscaler, -0.7 % time, and the ISA lint
 // (tools/lint_mfma_srcc.py) caught the asm overwriting an MFMA's SrcC quad two instructions behind it with no wait states:

@@ -46,3 +46,30 @@ def test_gelu_far_away_and_not_finite():
         ends = gelu(np.array([np.inf, -np.inf, np.nan, 0.0], F))
     # as x (1 + erf) / 2 gives them
     assert ends[0] == np.inf and np.isnan(ends[1]) and np.isnan(ends[2]) and ends[3] == 0
+
+
+def test_stated_bounds_of_the_packed_polynomial():
+    """csam_common.h states of csam_gelu_poly2, the detector's GELU: 4.1e-5 below 3, 8.1e-5 up to the clamp, 1.31e-6 |x| beyond.  Every fp32
+    value about the largest error, in the order that the kernel evaluates."""
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "crowdsam_amd", "csrc", "csam_common.h")).read()
+    body = src[src.index("csam_gelu_poly2(float2_t x)"):]
+    c = F(re.search(r"const float c = ([0-9.]+)f;", body)[1])
+    k = [F(v) for v in re.search(r"k\[9\] = \{(.*?)\};", body, re.S)[1].replace("f", "").split(",")]
+
+    def fma(a, b, d):
+        return (a.astype(np.float64) * b.astype(np.float64) + np.float64(d)).astype(F)
+
+    def off(x):
+        xc = np.clip(x, -c, c)
+        u, r = xc * xc, np.full_like(x, k[0])
+        for v in k[1:]:
+            r = fma(r, u, v)
+        return np.abs((x * fma(xc, r, F(0.5))).astype(np.float64) - exact(x))
+
+    about = np.arange(F(4.2).view(np.int32), F(4.4).view(np.int32), dtype=np.int32).view(F)
+    x = np.concatenate((np.linspace(-4.4, 4.4, 880_001).astype(F), about, -about))
+    e = off(x)
+    assert 8.0e-5 < float(e.max()) <= 8.1e-5 and float(e[np.abs(x) < 3].max()) <= 4.1e-5
+    far = np.geomspace(4.4, 6e4, 2001).astype(F)
+    assert bool((off(far) <= 8.1e-5 + 1.31e-6 * far).all()) and bool((off(-far) <= 8.1e-5 + 1.31e-6 * far).all())
+    assert bool((off(-far[far > 20]) <= 1.31e-6 * far[far > 20]).all())
