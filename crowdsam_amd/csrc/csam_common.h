@@ -94,7 +94,7 @@ __device__ __forceinline__ float csam_gelu_erf(float x) {
 }
 // Packed-fp32 polynomial GELU for fp16-bound outputs (the fused upscaler, which PMC shows VALU-bound on GELU):
 //   Phi(x) ~ 0.5 + xc * R(xc^2),  xc = clamp(x, +-4.4),  R = degree-8 minimax fit with Phi(4.4) = 1 (tools/fit_gelu_poly.py).
-// In fp32: |gelu error| <= 4.1e-5 for |x| < 3, <= 8.1e-5 up to the clamp (at x = -4.34; 4.5e-5 on the fit's grid), and 1.31e-6 |x|
+// In fp32: |gelu error| <= 4.1e-5 for |x| < 3, <= 8.1e-5 up to the clamp (at x = -4.34; 4.5e-5 on the fit's grid), and 1.4e-6 |x|
 // beyond it, where Phi stays 1.0000013 or -1.3e-6.  That is below half an fp16 step of the result where the result is over 0.17; of the
 // small negative results it is many steps, and x far below -4.4 gives a small POSITIVE value.
 // 13 instructions per PAIR (v_med3 x2, 11 v_pk_*_f32), no transcendental, against ~22 issue slots per element for the erf form above.

@@ -52,7 +52,7 @@ extern "C" {
 #define CSAM_ERR_WORKSPACE (-3)
 #define CSAM_ACT_NONE 0
 #define CSAM_ACT_GELU 1 /* erf GELU (nn.GELU default): fp32 outputs use erf (A&S 7.1.26, |err| <= 1.5e-7); fp16 outputs and
-                          * the fused upscaler use a minimax polynomial of Phi (|err| <= 8.1e-5, and 1.31e-6 |x| where |x| > 4.4:
+                          * the fused upscaler use a minimax polynomial of Phi (|err| <= 8.1e-5, and 1.4e-6 |x| where |x| > 4.4:
                           * below half an fp16 step of results over 0.17, more than that of small negative ones;
                           * csam_common.h csam_gelu_poly2, tools/fit_gelu_poly.py).  csam_mx_gemm's 16-bit outputs: within 6e-6 of
                           * the result down to x = -6.25, 1.3e-9 below */

@@ -49,7 +49,7 @@ def test_gelu_far_away_and_not_finite():
 
 
 def test_stated_bounds_of_the_packed_polynomial():
-    """csam_common.h states of csam_gelu_poly2, the detector's GELU: 4.1e-5 below 3, 8.1e-5 up to the clamp, 1.31e-6 |x| beyond.  Every fp32
+    """csam_common.h states of csam_gelu_poly2, the detector's GELU: 4.1e-5 below 3, 8.1e-5 up to the clamp, 1.4e-6 |x| beyond.  Every fp32
     value about the largest error, in the order that the kernel evaluates."""
     src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "crowdsam_amd", "csrc", "csam_common.h")).read()
     body = src[src.index("csam_gelu_poly2(float2_t x)"):]
@@ -71,5 +71,5 @@ def test_stated_bounds_of_the_packed_polynomial():
     e = off(x)
     assert 8.0e-5 < float(e.max()) <= 8.1e-5 and float(e[np.abs(x) < 3].max()) <= 4.1e-5
     far = np.geomspace(4.4, 6e4, 2001).astype(F)
-    assert bool((off(far) <= 8.1e-5 + 1.31e-6 * far).all()) and bool((off(-far) <= 8.1e-5 + 1.31e-6 * far).all())
-    assert bool((off(-far[far > 20]) <= 1.31e-6 * far[far > 20]).all())
+    assert bool((off(far) <= 8.1e-5 + 1.4e-6 * far).all()) and bool((off(-far) <= 8.1e-5 + 1.4e-6 * far).all())
+    assert bool((off(-far[far > 20]) <= 1.4e-6 * far[far > 20]).all())
