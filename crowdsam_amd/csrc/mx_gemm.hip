@@ -205,6 +205,12 @@ __device__ __forceinline__ intx8 mx_frag(const void* lo, const void* hi) {
   return intx8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
 }
 
+template <int... I, typename F>
+__device__ __forceinline__ void mx_for_each(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F>
+__device__ __forceinline__ void mx_for(F f) { mx_for_each(std::make_integer_sequence<int, N>{}, f); }
+#define MX_C(x) (std::integral_constant<int, (x)>{})
+
 // An E4M3 part whose products are summed as fp32 sums them: both operands become bf16, which holds a scaled code of either format exactly,
 // and four 32x32x16 instructions take the part.  Lane group g then holds codes 16g .. 16g + 15 of both blocks of the part: A's fragment is
 // that already, W's group has 32 codes of one block and swaps halves with the other group, as the two groups' scales do.
@@ -224,10 +230,11 @@ __device__ __forceinline__ void mx_scales(int s, unsigned (&byte)[2]) {        /
 }
 // a NaN block, or codes whose scale is so near the ends of the range that their product with it may not be a normal bf16
 __device__ __forceinline__ bool mx_far(unsigned byte, unsigned codes) { return (byte == 255u) | ((byte - 32u >= 192u) & (codes != 0u)); }
-template <int KK>
-__device__ __forceinline__ bool mx_bf16_a(const intx8& f, int s, mx_bf8 (&out)[4]) {
-  unsigned byte[2];
-  mx_scales<KK>(s, byte);
+__device__ __forceinline__ bool mx_far_a(const intx8& f, const unsigned (&byte)[2]) {
+  return mx_far(byte[0], (unsigned)(f[0] | f[1] | f[2] | f[3])) | mx_far(byte[1], (unsigned)(f[4] | f[5] | f[6] | f[7]));
+}
+// the codes times their scales (byte 127: as they are)
+__device__ __forceinline__ void mx_bf16_a(const intx8& f, const unsigned (&byte)[2], mx_bf8 (&out)[4]) {
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const float sc = __builtin_bit_cast(float, byte[m / 2] << 23);
@@ -238,23 +245,51 @@ __device__ __forceinline__ bool mx_bf16_a(const intx8& f, int s, mx_bf8 (&out)[4
       out[m][4 * d] = lo[0], out[m][4 * d + 1] = lo[1], out[m][4 * d + 2] = hi[0], out[m][4 * d + 3] = hi[1];
     }
   }
-  return mx_far(byte[0], (unsigned)(f[0] | f[1] | f[2] | f[3])) | mx_far(byte[1], (unsigned)(f[4] | f[5] | f[6] | f[7]));
 }
-template <int KK>
-__device__ __forceinline__ bool mx_bf16_w(const intx8& f, int s, mx_bf8 (&out)[4]) {
-  unsigned byte[2];
-  mx_scales<KK>(s, byte);
-  unsigned q[4] = {(unsigned)f[0], (unsigned)f[1], (unsigned)f[2], (unsigned)f[3]};      // the first 16 codes, the others
-  mx_swap32(q[0], q[2]);                                                                   // of the part's first block, of its second
+__device__ __forceinline__ void mx_swap_w(intx8& f) {                                     // the first 16 codes, the others
+  unsigned q[4] = {(unsigned)f[0], (unsigned)f[1], (unsigned)f[2], (unsigned)f[3]};      // of the part's first block, of its second
+  mx_swap32(q[0], q[2]);
   mx_swap32(q[1], q[3]);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) f[m] = (int)q[m];
+}
+__device__ __forceinline__ bool mx_far_w(const intx8& f, const unsigned (&byte)[2]) {
+  return mx_far(byte[0], (unsigned)(f[0] | f[1])) | mx_far(byte[1], (unsigned)(f[2] | f[3]));
+}
+__device__ __forceinline__ void mx_bf16_w(const intx8& f, const unsigned (&byte)[2], mx_bf8 (&out)[4]) {
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const float sc = __builtin_bit_cast(float, byte[m / 2] << 23);
-    const mx_bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 1);
-    const mx_bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[m], sc, 3);
+    const mx_bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)f[m], sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)f[m], sc, 1);
+    const mx_bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)f[m], sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)f[m], sc, 3);
     out[m] = mx_bf8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   }
-  return mx_far(byte[0], q[0] | q[1]) | mx_far(byte[1], q[2] | q[3]);
+}
+// acc + t 2^(a + w - 254): the sum of a block's products of bare codes, by the blocks' E8M0 bytes
+__device__ __forceinline__ float mx_add_scaled(float acc, float t, int a, int w) {
+  return acc + (max(a, w) == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(t, a + w - 254));
+}
+// A part with far blocks: the bare codes are multiplied (every product is a multiple of 2^-10 below 2^12), each block's sum then takes its
+// scales, so that whatever the scales are nothing is lost but what fp32 does not hold.
+__device__ __forceinline__ void mx_far_part(const intx8& w, const unsigned (&wbyte)[2], const intx8& a, const unsigned (&abyte)[2],
+                                            floatx16& acc, int g) {
+  const unsigned bare[2] = {127u, 127u};
+  mx_bf8 ab[4], wb[4];
+  mx_bf16_a(a, bare, ab);
+  mx_bf16_w(w, bare, wb);
+  mx_for<2>([&](auto f_) {
+    constexpr int f = decltype(f_)::value;
+    floatx16 t = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[2 * f], ab[2 * f], t, 0, 0, 0);
+    t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[2 * f + 1], ab[2 * f + 1], t, 0, 0, 0);
+    int from = 4 * g;
+    asm volatile("" : "+v"(from));                         // fetched anew for every tile: kept, W's scales would take 64 registers
+    mx_for<16>([&](auto e_) {                              // register e holds W's row 8 (e / 4) + 4g + e % 4
+      constexpr int e = decltype(e_)::value;
+      acc[e] = mx_add_scaled(acc[e], t[e], (int)abyte[f], __shfl((int)wbyte[f], from + 8 * (e / 4) + e % 4));
+      if constexpr (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);       // (four in flight: registers)
+    });
+  });
 }
 
 // --------------------------------------------------------------------------------------------------------------- tiled form
@@ -294,12 +329,6 @@ template <int RB>
 __device__ __forceinline__ int mx_lds_piece(int r, int c) {
   return RB == 128 ? r * 128 + ((c ^ ((r >> 1) & 7)) << 4) : r * 64 + ((c ^ ((r >> 2) & 3)) << 4);
 }
-
-template <int... I, typename F>
-__device__ __forceinline__ void mx_for_each(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
-template <int N, typename F>
-__device__ __forceinline__ void mx_for(F f) { mx_for_each(std::make_integer_sequence<int, N>{}, f); }
-#define MX_C(x) (std::integral_constant<int, (x)>{})
 
 template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS, bool EXACT = false>
 __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 ? 1 : 2) void mx_gemm_kernel(MxGemmArgs p) {
@@ -391,24 +420,33 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
   };
   // part h: matrix instructions on scale set ss; between them the reads of part rh (scale set rs) from stage rslot and the DMAs
   // [d0, d1) of step dt into stage dslot.  The reads go first, so that they are done when the part is.
-  auto part = [&](auto h_, auto ss_, auto rh_, auto rs_, int rslot, auto d0_, auto d1_, int dslot, int dt) {
+  auto part = [&](auto h_, auto ss_, auto rh_, auto rs_, int rslot, auto d0_, auto d1_, int dslot, int dt) __attribute__((always_inline)) {
     constexpr int h = decltype(h_)::value, ss = decltype(ss_)::value, rh = decltype(rh_)::value;
     constexpr int d0 = decltype(d0_)::value, d1 = decltype(d1_)::value;
     constexpr int S = (rh & 1) == 0 ? NSC : 0, NR = NF + S, ND = d1 - d0;
     mx_bf8 ab[EXACT ? MI : 1][4], wb[EXACT ? NI : 1][4];
+    unsigned abyte[EXACT ? MI : 1][2], wbyte[EXACT ? NI : 1][2];
     bool far = false;
-    if constexpr (EXACT) {                                // (parts with scales at the ends of the range take the scaled instruction)
+    if constexpr (EXACT) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) far |= mx_bf16_a<(h & 1)>(af[h & 1][i], sa[ss][i], ab[i]);
+      for (int i = 0; i < MI; ++i) mx_scales<(h & 1)>(sa[ss][i], abyte[i]), far |= mx_far_a(af[h & 1][i], abyte[i]);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) far |= mx_bf16_w<(h & 1)>(wf[h & 1][j], sw[ss][j], wb[j]);
+      for (int j = 0; j < NI; ++j) {
+        mx_scales<(h & 1)>(sw[ss][j], wbyte[j]);
+        mx_swap_w(wf[h & 1][j]);
+        far |= mx_far_w(wf[h & 1][j], wbyte[j]);
+      }
       far = __builtin_amdgcn_ballot_w64(far) != 0;        // uniform: matrix instructions do not heed the lanes' mask
     }
     constexpr int GAPS = NQ < 4 ? NQ : 4, RPG = (NR + GAPS - 1) / GAPS, G0 = NQ > 4 ? 2 : 0;
-    auto run = [&](auto bf_) {
+    constexpr int SCALED = 0, AS_BF16 = 1, FAR = 2;
+    auto run = [&](auto form_) __attribute__((always_inline)) {
+      constexpr int form = decltype(form_)::value;
       mx_for<NQ>([&](auto q_) {
         constexpr int q = decltype(q_)::value, i = q / NI, j = q % NI;
-        if constexpr (decltype(bf_)::value) {
+        if constexpr (form == FAR) {
+          mx_far_part(wf[h & 1][j], wbyte[j], af[h & 1][i], abyte[i], acc[i][j], g);
+        } else if constexpr (form == AS_BF16) {
 #pragma unroll
           for (int m = 0; m < 4; ++m) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j][m], ab[i][m], acc[i][j], 0, 0, 0);
         } else {
@@ -426,8 +464,19 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
         __builtin_amdgcn_sched_barrier(0);
       });
     };
-    if (EXACT && !far) run(std::integral_constant<bool, EXACT>{});
-    else run(std::false_type{});
+    if constexpr (EXACT) {
+      if (!far) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) mx_bf16_a(af[h & 1][i], abyte[i], ab[i]);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) mx_bf16_w(wf[h & 1][j], wbyte[j], wb[j]);
+        run(MX_C(AS_BF16));
+      } else {
+        run(MX_C(FAR));
+      }
+    } else {
+      run(MX_C(SCALED));
+    }
   };
   constexpr int FIRST = (PER + NH - 1) / NH;              // DMAs of a stage that its first (the last) part issues
   mx_for<NS - 1>([&](auto s_) { mx_for<PER>([&](auto d_) { dma(d_, decltype(s_)::value, min(decltype(s_)::value, nt - 1)); }); });
@@ -439,7 +488,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
   mx_for<NF>([&](auto k_) { read(k_, MX_C(0), 0); });
   // step t, t % UN = u: stages and scale sets are constants of the unrolled loop.  Scale sets: by step (NH = 2) or by pair of parts.
   constexpr int UN = NH == 2 && NS % 2 ? 2 * NS : NS;
-  auto step = [&](int t, auto u_) {
+  auto step = [&](int t, auto u_) __attribute__((always_inline)) {
     constexpr int u = decltype(u_)::value, slot = u % NS, next = (u + 1) % NS, prev = (u + NS - 1) % NS, us = u & 1;
     mx_for<NH - 1>([&](auto h_) {
       constexpr int h = decltype(h_)::value;

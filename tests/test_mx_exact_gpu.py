@@ -1,0 +1,103 @@
+"""hip.mx_gemm of an E4M3 operand where the scaled matrix instruction drops bits: sums that fp32 holds exactly in any order and that need
+bits far below 2^-13 of a neighbouring product."""
+import pytest
+import torch
+
+import mx_ref
+from test_mx_gpu import gen
+
+pytestmark = pytest.mark.gpu
+
+
+def fine(m, n, k, seed):
+    """(qa, qw, float64 product).  Of 16 neighbours of a row of A one is +-256, the others are multiples of 2^-9 below 2^-3; W holds +-1/2 and
+    +-1.  Every product is a multiple of 2^-10 and every sum of k <= 512 is below 32 x 256 + 512 / 8 < 2^14: 24 bits, exact in any order.
+    The matrix instruction keeps 2^-5 of a group that 256 leads."""
+    from crowdsam_amd import hip
+    g = gen(seed)
+    small = torch.cat((torch.arange(8.0) * 2.0 ** -9, (8 + torch.arange(8.0)) * 2.0 ** -8, (8 + torch.arange(8.0)) * 2.0 ** -7))
+    a = small[torch.randint(0, len(small), (m, k), generator=g)]
+    at = torch.randint(0, 16, (m, -(-k // 16)), generator=g) + 16 * torch.arange(-(-k // 16))
+    a.scatter_(1, at.clamp(max=k - 1), 256.0)
+    a = a * (torch.randint(0, 2, (m, k), generator=g) * 2 - 1)
+    w = torch.tensor([0.5, -0.5, 1.0, -1.0])[torch.randint(0, 4, (n, k), generator=g)]
+    w[:, ::32] = 1.0
+    qa, qw = hip.mx_quantize(a.cuda(), "fp8"), hip.mx_quantize(w.cuda(), "fp4")
+    assert torch.equal(mx_ref.values(qa), a.double()) and torch.equal(mx_ref.values(qw), w.double())
+    return qa, qw, a.double() @ w.double().t()
+
+
+def scaled(q, powers, rows=None):
+    """``q`` with the scale bytes of its blocks moved by ``powers`` [groups of 128 columns], of all rows or those given (blocks behind K
+    stay)."""
+    groups, m, _ = q.scales.shape
+    by = torch.as_tensor(powers, dtype=torch.int32).view(-1, 1, 1).expand(groups, m, 4).clone()
+    by[(torch.arange(groups * 4) >= -(-q.K // 32)).view(groups, 1, 4).expand_as(by)] = 0
+    if rows is not None:
+        keep = torch.ones(m, dtype=torch.bool)
+        keep[rows] = False
+        by[:, keep] = 0
+    s = q.scales.int() + by.to(q.scales.device)
+    assert 0 <= int(s.min()) and int(s.max()) < 255
+    return q._replace(scales=s.to(torch.uint8))
+
+
+# one row and few rows; 64-wide tiles; 128-wide tiles, whole and ragged
+SHAPES = [(1, 64, 256), (3, 130, 512), (16, 260, 500), (33, 40, 256), (200, 300, 512), (511, 130, 300), (2048, 2048, 256), (2100, 2001, 300)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_fp32_results_lose_nothing(cuda, m, n, k):
+    from crowdsam_amd import hip
+    qa, qw, ref = fine(m, n, k, m + n)
+    assert torch.equal(hip.mx_gemm(qa, qw, out_dtype=torch.float32).cpu().double(), ref)
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_fp32_results_lose_nothing_at_any_scale(cuda, m, n, k):
+    """The same values with their scales moved to the ends of the range, undone in the other operand: the same bits."""
+    from crowdsam_amd import hip
+    qa, qw, ref = fine(m, n, k, m + n + 1)
+    groups = qa.scales.shape[0]
+    by = torch.tensor([0, 125, -120, 97])[torch.arange(groups) % 4]
+    out = hip.mx_gemm(scaled(qa, by), scaled(qw, -by), out_dtype=torch.float32)
+    assert torch.equal(out.cpu().double(), ref)
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_rows_at_the_ends_of_the_range_leave_the_others_whole(cuda, m, n, k):
+    """Rows of A and of W with far scales of their own: their results are moved by the same power of two, the others keep every bit.  A row
+    that is too small for fp32 becomes what fp32 makes of it; a NaN block is its row's alone."""
+    from crowdsam_amd import hip
+    qa, qw, ref = fine(m, n, k, m + n + 2)
+    groups = qa.scales.shape[0]
+    up, down = m // 2, m - 1
+    qa = scaled(qa, [100] * groups, [up])
+    if down != up:
+        qa = scaled(qa, [-100] * groups, [down])
+    qw = scaled(qw, [-110] * groups, [n // 2])
+    power = torch.zeros(m, n, dtype=torch.float64)
+    power[up] += 100
+    if down != up:
+        power[down] -= 100
+    power[:, n // 2] -= 110
+    want = (ref * torch.exp2(power)).float()
+    out = hip.mx_gemm(qa, qw, out_dtype=torch.float32).cpu()
+    tiny = want.abs() < 2.0 ** -126                        # (fp32 may flush them)
+    assert torch.equal(out[~tiny], want[~tiny]) and float(out[tiny].abs().max() if tiny.any() else 0) < 2.0 ** -125
+    s = qw.scales.clone()
+    s[1, 0, 2] = 255
+    out = hip.mx_gemm(qa, qw._replace(scales=s), out_dtype=torch.float32).cpu()
+    assert bool(out[:, 0].isnan().all()) and torch.equal(out[:, 1:][~tiny[:, 1:]], want[:, 1:][~tiny[:, 1:]])
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_the_cut_stays_in_its_bound_and_shows(cuda, m, n, k):
+    """``cut``: each of the 15 neighbours of a group loses less than 2^-13 of the group's largest product, 2^-5 here, in ceil(k / 16) groups.
+    Many rows show it, so the tests above can tell the two apart."""
+    from crowdsam_amd import hip
+    qa, qw, ref = fine(m, n, k, m + n)
+    d = (hip.mx_gemm(qa, qw, out_dtype=torch.float32, cut=True).cpu().double() - ref).abs()
+    assert float(d.max()) <= 15 * 2.0 ** -5 * -(-k // 16)
+    if m >= 200:
+        assert float(d.max()) > 0
