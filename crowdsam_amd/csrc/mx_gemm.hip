@@ -551,8 +551,25 @@ __global__ __launch_bounds__(WGM * WGN * 64, (TM / WGM) * (TN / WGN) > 128 * 64 
 // 16x16x128 instruction j of a step takes blocks 2g + j: lane group g = 0 .. 3 supplies the scales of its two blocks (one 16-bit load);
 // an E4M3 operand's lane group holds half (g & 1) of logical blocks g / 2 and 2 + g / 2.
 // Bound by the latency of a wave's few loads: 1 x 4096 x 1024 E4M3 3.3 us, 32 x 4096 x 4096 E2M1 5.7 us (1.6 TB/s of weights).
-template <int FA, int MT, int NW>
+// EXACT (an E4M3 operand whose products keep every bit): the bare codes as bf16, a block of 32 per 16x16x32 instruction, its sum scaled by
+// the blocks' bytes.  A lane's two blocks of each operand are shared out among the lane groups, 8 codes each, by lane swaps.  us, the scaled
+// instruction / so / 64x64 tiles: 1 x 1024 x 4096 4.4 / 6.6 / 24.5, 16 x 4096 x 4096 6.0 / 8.1 / 25, 32 x 4096 x 4096 7.9 / 11.2 / 25,
+// 224 x 256 x 1024 3.8 / 4.5 / 9.0.
+__device__ __forceinline__ void mx_swap16(unsigned& a, unsigned& b) {          // a's odd rows of 16 lanes for b's even ones
+  const auto p = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = p[0];
+  b = p[1];
+}
+// x[d] of lane group g for x[g] of lane group d
+__device__ __forceinline__ void mx_turn(unsigned& x0, unsigned& x1, unsigned& x2, unsigned& x3) {
+  mx_swap32(x0, x2);
+  mx_swap32(x1, x3);
+  mx_swap16(x0, x1);
+  mx_swap16(x2, x3);
+}
+template <int FA, int MT, int NW, bool EXACT = false>
 __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(MxGemmArgs p) {
+  static_assert(!EXACT || FA == CSAM_MX_FP8, "E2M1 products lose nothing");
   __shared__ floatx4 part[NW][MT][64];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -565,30 +582,80 @@ __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(MxGemmArgs p) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const long row = min(bm0 + i * 16 + r, p.M - 1);
-    ap[i] = p.A + row * p.lda + (FA == CSAM_MX_FP8 ? (g >> 1) * 64 + (g & 1) * 16 : g * 32);
-    asp[i] = p.As + row * 4 + (long)(g >> 1) * p.a_ss + 2 * (g & 1);
+    ap[i] = p.A + row * p.lda + (EXACT ? g * 64 : FA == CSAM_MX_FP8 ? (g >> 1) * 64 + (g & 1) * 16 : g * 32);
+    asp[i] = p.As + row * 4 + (EXACT ? 0 : (long)(g >> 1) * p.a_ss + 2 * (g & 1));
   }
   floatx4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   const int nt = p.Kp / 256;
   for (int t = wave; t < nt; t += NW) {
-    const intx8 w0 = mx_frag(wp + (long)t * 128), w1 = mx_frag(wp + (long)t * 128 + 16);
-    const int sw = *(const unsigned short*)(wsp + 2L * t * p.w_ss);
+    if constexpr (EXACT) {
+      unsigned w[2][4], sw[2][4];                          // of W: block 2b + j's codes 8g .. 8g + 7 at [j][b]; rows 4g + e's scales [half][e]
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int sa = *(const unsigned short*)(asp[i] + 2L * t * p.a_ss);
-      intx8 a0, a1;
-      if constexpr (FA == CSAM_MX_FP8) {
-        const uint8_t* a = ap[i] + (long)t * 256;          // logical block g of instruction j = block 2g + j of the step
-        a0 = mx_frag(a, a + 128);
-        a1 = mx_frag(a + 32, a + 160);
-      } else {
-        a0 = mx_frag(ap[i] + (long)t * 128);
-        a1 = mx_frag(ap[i] + (long)t * 128 + 16);
+      for (int j = 0; j < 2; ++j) {
+        const uintx4 c = *(const uintx4*)(wp + (long)t * 128 + 16 * j);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) w[j][d] = c[d];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sw[j][e] = *(const unsigned*)(p.Ws + (2L * t + j) * p.w_ss + 4L * min(bn0 + 4 * g + e, p.N - 1));
       }
-      acc[i] = mx_mfma16<FA, 0>(w0, a0, acc[i], sw, sa);
-      acc[i] = mx_mfma16<FA, 1>(w1, a1, acc[i], sw, sa);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mx_turn(w[j][0], w[j][1], w[j][2], w[j][3]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        unsigned a[2][8], sa[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sa[j] = *(const unsigned*)(asp[i] + (2L * t + j) * p.a_ss);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uintx4 c = *(const uintx4*)(ap[i] + (long)t * 256 + 32 * j + 16 * q);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) a[j][4 * q + d] = c[d];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mx_turn(a[j][0], a[j][2], a[j][4], a[j][6]);     // then block 2b + j's codes 8g .. 8g + 3 at [j][2b], the next four behind
+          mx_turn(a[j][1], a[j][3], a[j][5], a[j][7]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const mx_bf2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[j][2 * b], 1.f, false), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[j][2 * b], 1.f, true);
+            const mx_bf2 a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[j][2 * b + 1], 1.f, false), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a[j][2 * b + 1], 1.f, true);
+            const mx_bf2 w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j][b], 1.f, 0), w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j][b], 1.f, 1);
+            const mx_bf2 w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j][b], 1.f, 2), w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j][b], 1.f, 3);
+            const floatx4 v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf8{w0[0], w0[1], w1[0], w1[1], w2[0], w2[1], w3[0], w3[1]},
+                                                                      mx_bf8{a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]},
+                                                                      floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            const int at = 8 * (2 * (b & 1) + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[i][e] = mx_add_scaled(acc[i][e], v[e], (int)(sa[b >> 1] >> at & 255u), (int)(sw[b >> 1][e] >> at & 255u));
+          }
+        }
+      }
+    } else {
+      const intx8 w0 = mx_frag(wp + (long)t * 128), w1 = mx_frag(wp + (long)t * 128 + 16);
+      const int sw = *(const unsigned short*)(wsp + 2L * t * p.w_ss);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int sa = *(const unsigned short*)(asp[i] + 2L * t * p.a_ss);
+        intx8 a0, a1;
+        if constexpr (FA == CSAM_MX_FP8) {
+          const uint8_t* a = ap[i] + (long)t * 256;        // logical block g of instruction j = block 2g + j of the step
+          a0 = mx_frag(a, a + 128);
+          a1 = mx_frag(a + 32, a + 160);
+        } else {
+          a0 = mx_frag(ap[i] + (long)t * 128);
+          a1 = mx_frag(ap[i] + (long)t * 128 + 16);
+        }
+        acc[i] = mx_mfma16<FA, 0>(w0, a0, acc[i], sw, sa);
+        acc[i] = mx_mfma16<FA, 1>(w1, a1, acc[i], sw, sa);
+      }
     }
   }
 #pragma unroll
@@ -600,6 +667,14 @@ __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(MxGemmArgs p) {
     for (int w = 1; w < NW; ++w) v += part[w][i][lane];
     mx_epilogue4(p, bm0 + i * 16 + r, bn0 + 4 * g, v);
   }
+}
+
+template <int FA, bool EXACT>
+int mx_rows(hipStream_t st, const MxGemmArgs& p, long t16) {
+  if (t16 <= 256 || p.M <= 16) mx_gemm_rows_kernel<FA, 1, 4, EXACT><<<(unsigned)t16, 256, 0, st>>>(p);
+  else mx_gemm_rows_kernel<FA, 2, 4, EXACT><<<(unsigned)((long)csam_cdiv(p.M, 32) * csam_cdiv(p.N, 16)), 256, 0, st>>>(p);
+  CSAM_LAUNCH_CHECK("csam_mx_gemm");
+  return CSAM_OK;
 }
 
 template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS, bool EXACT = false>
@@ -629,22 +704,19 @@ int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
 //   16384 x 4096 x 4096    128x128 218, 256x256 183                   128x256 292, 256x256 267
 template <int FA>
 int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
+  const long t16 = (long)csam_cdiv(p.M, 16) * csam_cdiv(p.N, 16);
+  const bool few = p.M <= 16 || t16 <= 512;
   if constexpr (FA == CSAM_MX_FP8) {
     // fp32 results keep what the scaled instruction drops, unless the caller lets it go.  us to fp32 (M x N x K), as bf16 / scaled to
     // fp16, the conversion to bf16 taking most of the difference: 224 x 2048 x 1024 9.4 / 4.9, 5330 x 4096 x 1024 75 / 34;
     // error in norm 7e-9 / 4.5e-6 before the rounding.
     if (p.c_dt == CSAM_DT_F32 && !p.cut) {
+      if (few) return mx_rows<FA, true>(st, p, t16);
       if ((long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128) >= 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 128, true>(st, p);
       return mx_tiles<FA, 64, 64, 2, 2, 4, 128, true>(st, p);
     }
   }
-  const long t16 = (long)csam_cdiv(p.M, 16) * csam_cdiv(p.N, 16);
-  if (p.M <= 16 || t16 <= 512) {
-    if (t16 <= 256 || p.M <= 16) mx_gemm_rows_kernel<FA, 1, 4><<<(unsigned)t16, 256, 0, st>>>(p);
-    else mx_gemm_rows_kernel<FA, 2, 4><<<(unsigned)((long)csam_cdiv(p.M, 32) * csam_cdiv(p.N, 16)), 256, 0, st>>>(p);
-    CSAM_LAUNCH_CHECK("csam_mx_gemm");
-    return CSAM_OK;
-  }
+  if (few) return mx_rows<FA, false>(st, p, t16);
   const long t256 = (long)csam_cdiv(p.M, 256) * csam_cdiv(p.N, 256), rounds = (t256 + 255) / 256;
   const bool brief = p.Kp <= 1024;
   const bool large = brief ? t256 >= 240 && rounds == 1 : rounds >= 4 || t256 * 4 >= rounds * 256 * 3;

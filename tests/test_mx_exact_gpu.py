@@ -42,8 +42,9 @@ def scaled(q, powers, rows=None):
     return q._replace(scales=s.to(torch.uint8))
 
 
-# one row and few rows; 64-wide tiles; 128-wide tiles, whole and ragged
-SHAPES = [(1, 64, 256), (3, 130, 512), (16, 260, 500), (33, 40, 256), (200, 300, 512), (511, 130, 300), (2048, 2048, 256), (2100, 2001, 300)]
+# one row and few rows (the direct form with one and with two tiles of 16 rows); 64-wide tiles; 128-wide tiles, whole and ragged
+SHAPES = [(1, 64, 256), (3, 130, 512), (16, 260, 500), (33, 40, 256), (200, 300, 512), (511, 130, 300), (2048, 2048, 256), (2100, 2001, 300),
+          (1, 4096, 512), (7, 1, 32), (100, 1000, 300), (300, 900, 300)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
