@@ -12,6 +12,7 @@
 #define CSAM_MX_FP4 0
 #define CSAM_MX_FP8 1
 #define CSAM_MX_CUT 16
+#define CSAM_MX_WHOLE 32
 
 typedef __bf16 bf16_t;
 typedef unsigned uintx2 __attribute__((ext_vector_type(2)));

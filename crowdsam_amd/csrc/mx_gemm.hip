@@ -6,9 +6,10 @@
 // instructions read neighbouring blocks 2g, 2g + 1 and its two scale bytes are one aligned 16-bit load.  An E4M3 operand is spread
 // differently: lane group g holds halves g (16 codes) of BOTH blocks.
 // What the instruction keeps: E2M1 products are summed as fp32 sums them.  With an E4M3 operand it lines 16 neighbouring products up to
-// the largest and drops bits below 2^-13 of that (measured: a product 2^-14 of its neighbour vanishes, one in the next 16 does not); on
-// gaussian rows the result is 4.5e-6 off in norm, against the 2e-2 that rounding the operand to E4M3 cost.  16-bit results take that; fp32
-// results only where the caller says so, otherwise both operands are multiplied as bf16, which holds them exactly.
+// the largest and drops bits below 2^-13 of that (measured: a product 2^-14 of its neighbour vanishes, one in the next 16 does not).  Of
+// the result's norm: 4.5e-6 on gaussian rows, 1.2e-5 where 4 of 1024 channels are thirty times the others, 6e-5 where the channels' sizes are
+// powers of two of a spread of 3; fp16's rounding is 2.1e-4, the rounding to E4M3 3e-2 to 6e-2.  16-bit results of many rows take that (a
+// third of the time) unless the caller forbids it; otherwise both operands are multiplied as bf16, which holds them exactly.
 // W rows are the instruction's row operand, A rows its columns: a lane ends up with 4 consecutive n of one row m.
 #include <type_traits>
 #include <utility>
@@ -24,7 +25,7 @@ struct MxGemmArgs {
   const float* bias;
   const void* R; long ldr; int r_dt;
   int act, M, N, Kp;
-  int cut;                                   // fp32 results may lose what the scaled instruction drops
+  int cut;                                   // CSAM_MX_CUT: results may lose what the scaled instruction drops; CSAM_MX_WHOLE: they may not
   int past;                                  // C's rows begin on lines of 128 bytes: large tiles may store past the caches
 };
 
@@ -707,10 +708,11 @@ int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
   const long t16 = (long)csam_cdiv(p.M, 16) * csam_cdiv(p.N, 16);
   const bool few = p.M <= 16 || t16 <= 512;
   if constexpr (FA == CSAM_MX_FP8) {
-    // fp32 results keep what the scaled instruction drops, unless the caller lets it go.  us to fp32 (M x N x K), as bf16 / scaled to
-    // fp16, the conversion to bf16 taking most of the difference: 224 x 2048 x 1024 9.4 / 4.9, 5330 x 4096 x 1024 75 / 34;
-    // error in norm 7e-9 / 4.5e-6 before the rounding.
-    if (p.c_dt == CSAM_DT_F32 && !p.cut) {
+    // What the scaled instruction drops is kept in fp32 results and in results of few rows, which are bound by latency, unless the caller
+    // lets it go, and in 16-bit results of many rows if the caller asks.  us to fp32 (M x N x K), as bf16 / scaled to fp16, the
+    // conversion to bf16 taking most of the difference: 224 x 2048 x 1024 9.4 / 4.9, 5330 x 4096 x 1024 75 / 34.
+    const bool whole = p.cut == CSAM_MX_WHOLE || (p.cut == 0 && (few || p.c_dt == CSAM_DT_F32));
+    if (whole) {
       if (few) return mx_rows<FA, true>(st, p, t16);
       if ((long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128) >= 256) return mx_tiles<FA, 128, 128, 2, 2, 2, 128, true>(st, p);
       return mx_tiles<FA, 64, 64, 2, 2, 4, 128, true>(st, p);
@@ -754,7 +756,8 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
   auto dt_ok = [](int dt) { return dt == CSAM_DT_F16 || dt == CSAM_DT_F32 || dt == CSAM_DT_BF16; };
   auto al = [](const void* q, long ld, int a) { return (uintptr_t)q % a == 0 && ld % a == 0; };
   CSAM_REQUIRE(dt_ok(c_dtype) && (!residual || dt_ok(r_dtype)), "csam_mx_gemm: bad dtype");
-  const int plain = act & ~CSAM_MX_CUT;
+  const int cut = act & (CSAM_MX_CUT | CSAM_MX_WHOLE), plain = act & ~cut;
+  CSAM_REQUIRE(cut != (CSAM_MX_CUT | CSAM_MX_WHOLE), "csam_mx_gemm: CSAM_MX_CUT and CSAM_MX_WHOLE exclude each other");
   CSAM_REQUIRE(plain == CSAM_ACT_NONE || plain == CSAM_ACT_GELU || plain == CSAM_ACT_RELU, "csam_mx_gemm: bad activation %d", act);
   CSAM_REQUIRE(lda >= (a_fmt == CSAM_MX_FP8 ? Kp : Kp / 2) && ldw >= Kp / 2, "csam_mx_gemm: code rows are shorter than %d padded columns", Kp);
   CSAM_REQUIRE(lda < (1 << 24) && ldw < (1 << 24), "csam_mx_gemm: code rows 16 MB apart or more");
@@ -763,6 +766,7 @@ extern "C" int csam_mx_gemm(void* stream, const void* A, long lda, const void* A
                "csam_mx_gemm: scale groups have to lie 4-byte aligned, at least 4 * rows bytes apart");
   CSAM_REQUIRE(ldc >= N && (!residual || ldr >= N), "csam_mx_gemm: an output row pitch is shorter than N");
   MxGemmArgs p = {(const uint8_t*)A, lda, (const uint8_t*)A_scales, a_scale_stride, (const uint8_t*)W, ldw, (const uint8_t*)W_scales,
-                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, act & ~CSAM_MX_CUT, M, N, Kp, act & CSAM_MX_CUT, al(C, ldc * (c_dtype == CSAM_DT_F32 ? 4 : 2), 128)};
+                  w_scale_stride, C, ldc, c_dtype, bias, residual, ldr, r_dtype, plain, M, N, Kp, cut,
+                  al(C, ldc * (c_dtype == CSAM_DT_F32 ? 4 : 2), 128)};
   return a_fmt == CSAM_MX_FP8 ? mx_gemm_launch<CSAM_MX_FP8>((hipStream_t)stream, p) : mx_gemm_launch<CSAM_MX_FP4>((hipStream_t)stream, p);
 }

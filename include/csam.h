@@ -119,7 +119,8 @@ int csam_linear_f32_batched(void* stream, const float* A, long lda, long strideA
 #define CSAM_DT_BF16 2
 #define CSAM_MX_FP4 0
 #define CSAM_MX_FP8 1
-#define CSAM_MX_CUT 16 /* or-ed to csam_mx_gemm's act */
+#define CSAM_MX_CUT 16   /* or-ed to csam_mx_gemm's act, one of them at most */
+#define CSAM_MX_WHOLE 32
 /* s = max(floor(log2 amax) - emax, -127) + 127 with emax 2 (E2M1) / 8 (E4M3), codes = x / 2^(s-127) rounded to nearest even and
  * saturated at 6 / 448.  A block that holds a NaN or an infinity gets s = 255 (and zero codes): all of it reads as NaN.  A block whose
  * amax is zero or subnormal gets s = 0. */
@@ -128,9 +129,11 @@ int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* c
 int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void* scales, long scale_stride, int fmt, void* y, long ldy,
                        int y_dtype, int M, int K);
 /* C[M,N] = act(A W^T + bias[n]) + residual[m,n]; A in either format, W in CSAM_MX_FP4, fp32 sums, one rounding to c_dtype.  bias
- * (fp32 [N]) and residual (f16 / f32 / bf16) may be NULL; C may be the residual itself.  An E4M3 A whose C is 16 bits wide is multiplied
- * by an instruction that drops bits below 2^-13 of the largest of 16 neighbouring products (4.5e-6 of the result's norm); for an fp32 C
- * nothing is dropped, at two to four times the time, unless act has CSAM_MX_CUT.  K is the unpadded width, at most 2^20; code rows
+ * (fp32 [N]) and residual (f16 / f32 / bf16) may be NULL; C may be the residual itself.  With an E4M3 A the scaled matrix instruction drops
+ * bits below 2^-13 of the largest of 16 neighbouring products (4.5e-6 of the result's norm for gaussian rows, 6e-5 where channels' sizes
+ * spread widely).  A 16-bit C of more than 16 rows and 512 tiles of 16 x 16 takes it, unless act has CSAM_MX_WHOLE; any other C loses
+ * nothing, at two to three times the time of many rows, unless act has CSAM_MX_CUT.
+ * K is the unpadded width, at most 2^20; code rows
  * less than 2^24 bytes apart. */
 int csam_mx_gemm(void* stream, const void* A, long lda, const void* A_scales, long a_scale_stride, int a_fmt, const void* W, long ldw,
                  const void* W_scales, long w_scale_stride, void* C, long ldc, int c_dtype, const float* bias, const void* residual,

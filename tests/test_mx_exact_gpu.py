@@ -102,3 +102,45 @@ def test_the_cut_stays_in_its_bound_and_shows(cuda, m, n, k):
     assert float(d.max()) <= 15 * 2.0 ** -5 * -(-k // 16)
     if m >= 200:
         assert float(d.max()) > 0
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_16_bit_results_lose_nothing_if_asked(cuda, out_dtype, m, n, k):
+    """cut=False: the exact sum, rounded once.  With no choice made that holds for few rows; many rows stay in the cut's bound."""
+    from crowdsam_amd import hip
+    qa, qw, ref = fine(m, n, k, m + n)
+    want = ref.to(out_dtype)                               # (ref is an fp32 value: one rounding)
+    assert torch.equal(hip.mx_gemm(qa, qw, out_dtype=out_dtype, cut=False).cpu(), want)
+    out = hip.mx_gemm(qa, qw, out_dtype=out_dtype).cpu()
+    if m <= 16 or -(-m // 16) * -(-n // 16) <= 512:
+        assert torch.equal(out, want)
+    else:
+        lost = 15 * 2.0 ** -5 * -(-k // 16)
+        assert float((out.double() - ref).abs().max()) <= lost + torch.finfo(out_dtype).eps / 2 * (float(ref.abs().max()) + lost)
+
+
+@pytest.mark.parametrize("m", [5, 300, 2100])
+def test_the_choice_with_an_epilogue(cuda, m):
+    """Bias, activation and residual behind a sum that lost nothing: integers of 1/4 that fp32 and fp16 hold, so the result is exact."""
+    from crowdsam_amd import hip
+    n, k = 2000, 256
+    g = gen(m)
+    a = torch.zeros(m, k)
+    a[:, 0], a[:, 1], a[:, 2] = 256.0, -256.0, 0.0625 * torch.randint(1, 16, (m,), generator=g)     # 2^-4 beside 2^8
+    w = torch.ones(n, k)
+    qa, qw = hip.mx_quantize(a.to(cuda), "fp8"), hip.mx_quantize(w.to(cuda), "fp4")
+    assert torch.equal(mx_ref.values(qa), a.double())
+    bias, res = 0.25 * torch.randint(-8, 9, (n,), generator=g), 0.25 * torch.randint(-8, 9, (m, n), generator=g)
+    out = hip.mx_gemm(qa, qw, bias=bias.float().to(cuda), act=hip.ACT_RELU, residual=res.half().to(cuda), cut=False)
+    ref = (a[:, 2].double()[:, None] + bias.double()).clamp(min=0) + res.double()
+    assert torch.equal(out.cpu(), ref.half())
+
+
+def test_the_choice_changes_nothing_for_e2m1(cuda):
+    from crowdsam_amd import hip
+    for m in (4, 700):
+        qa = hip.mx_quantize(torch.randn(m, 300, generator=gen(m)).to(cuda), "fp4")
+        qw = hip.mx_quantize(torch.randn(900, 300, generator=gen(1)).to(cuda), "fp4")
+        outs = [hip.mx_gemm(qa, qw, out_dtype=torch.float32, cut=cut) for cut in (None, False, True)]
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
