@@ -14,6 +14,9 @@
 #define CSAM_MX_CUT 16
 #define CSAM_MX_WHOLE 32
 
+// A launch has fewer than 2^32 work items (HIP's limit on grid times workgroup in one dimension)
+inline bool csam_launch_fits(long groups, int threads) { return groups <= 0xffffffffL / threads; }
+
 typedef __bf16 bf16_t;
 typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));

@@ -672,6 +672,7 @@ __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(MxGemmArgs p) {
 
 template <int FA, bool EXACT>
 int mx_rows(hipStream_t st, const MxGemmArgs& p, long t16) {
+  CSAM_REQUIRE(csam_launch_fits(t16, 256), "csam_mx_gemm: %d x %d is more than one launch takes", p.M, p.N);
   if (t16 <= 256 || p.M <= 16) mx_gemm_rows_kernel<FA, 1, 4, EXACT><<<(unsigned)t16, 256, 0, st>>>(p);
   else mx_gemm_rows_kernel<FA, 2, 4, EXACT><<<(unsigned)((long)csam_cdiv(p.M, 32) * csam_cdiv(p.N, 16)), 256, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_mx_gemm");
@@ -681,7 +682,7 @@ int mx_rows(hipStream_t st, const MxGemmArgs& p, long t16) {
 template <int FA, int TM, int TN, int WGM, int WGN, int NS, int KS, bool EXACT = false>
 int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
   const long grid = (long)csam_cdiv(p.M, TM) * csam_cdiv(p.N, TN);
-  CSAM_REQUIRE(grid < (1L << 31), "csam_mx_gemm: too many tiles");
+  CSAM_REQUIRE(csam_launch_fits(grid, WGM * WGN * 64), "csam_mx_gemm: %d x %d is more than one launch takes", p.M, p.N);
   mx_gemm_kernel<FA, TM, TN, WGM, WGN, NS, KS, EXACT><<<(unsigned)grid, WGM * WGN * 64, 0, st>>>(p);
   CSAM_LAUNCH_CHECK("csam_mx_gemm");
   return CSAM_OK;

@@ -240,6 +240,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void rms_norm_kernel(RmsAr
 template <typename T, int RK, int V, bool NT>
 int rms_launch_v(hipStream_t st, const RmsArgs& p) {
   const int chunks = csam_cdiv(p.Dp ? p.Dp : p.D, 8);      // of 8
+  CSAM_REQUIRE(chunks <= 256 ? csam_launch_fits(csam_cdiv(p.M, 4), 256) : csam_launch_fits(p.M, chunks <= 1024 ? 256 : 1024),
+               "csam_rms_norm: %d rows of %d are more than one launch takes", p.M, p.D);
 #define RMS_GO(NW, MAXC) rms_norm_kernel<T, RK, NW, MAXC * 8 / V, V, NT><<<csam_cdiv(p.M, NW == 1 ? 4 : 1), NW == 1 ? 256 : NW * 64, 0, st>>>(p)
   if (chunks <= 64) RMS_GO(1, 1);
   else if (chunks <= 128) RMS_GO(1, 2);
@@ -294,7 +296,7 @@ int csam_mx_quantize(void* stream, const void* x, long ldx, int x_dtype, void* c
   if (int rc = mx_check("csam_mx_quantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
   const int nseg = csam_cdiv(K, Q_COLS);
   const long grid = (long)nseg * csam_cdiv(M, 8);
-  CSAM_REQUIRE(grid < (1L << 31), "csam_mx_quantize: too many elements");
+  CSAM_REQUIRE(csam_launch_fits((long)nseg * csam_cdiv(M, 32), 256), "csam_mx_quantize: %d x %d is more than one launch takes", M, K);
   hipStream_t st = (hipStream_t)stream;
 #define GO(T, F)                                                                                                         \
   do {                                                                                                                   \
@@ -326,7 +328,8 @@ int csam_mx_dequantize(void* stream, const void* codes, long ldcodes, const void
   if (int rc = mx_check("csam_mx_dequantize", codes, ldcodes, scales, scale_stride, fmt, M, K)) return rc;
   const int nseg = csam_cdiv(K, Q_COLS);
   const long grid = (long)nseg * csam_cdiv(M, 8);
-  CSAM_REQUIRE(2 * grid < (1L << 31), "csam_mx_dequantize: too many elements");
+  CSAM_REQUIRE(csam_launch_fits((long)nseg * csam_cdiv(M, y_dtype == CSAM_DT_F32 ? 16 : 32), 256),
+               "csam_mx_dequantize: %d x %d is more than one launch takes", M, K);
   hipStream_t st = (hipStream_t)stream;
 #define GO(T, F)                                                                                                         \
   do {                                                                                                                   \

@@ -193,7 +193,7 @@ int rotary_launch(hipStream_t st, RotaryArgs& p) {
   p.by_token = recip((long)p.heads * p.units);
   p.by_pair = recip(p.P);
   const long grid = (long)csam_cdiv(p.T, p.tokens) * p.splits;
-  CSAM_REQUIRE(grid < (1L << 31), "csam_rotary: too many elements");
+  CSAM_REQUIRE(csam_launch_fits(grid, 256), "csam_rotary: %d tokens x %d heads of %d are more than one launch takes", p.T, H, p.hd);
   // Results beyond the L2s' size are stored past them (16384 tokens x 32 heads of 80, interleaved: 30.6 us, 27.7 so; of 128 with 64 pairs,
   // half: 53.5, 42.1), unless a run of a head ends inside a 64-byte line, which two stores then fill: those meet in the L2 (of 80 with 40
   // pairs, half: past the caches 61.8, 32.2 so).

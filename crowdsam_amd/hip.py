@@ -152,10 +152,14 @@ def lib():
     return _lib
 
 
+class ArgumentError(RuntimeError, ValueError):
+    """An entry refused its arguments."""
+
+
 def _check(rc, name):
     if rc != 0:
         msg = lib().csam_last_error().decode()
-        raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+        raise (ArgumentError if rc == -1 else RuntimeError)(f"{name} failed (rc={rc}): {msg}")
 
 
 def _ptr(t):
@@ -1358,7 +1362,8 @@ def mx_gemm(a, w, out=None, bias=None, act=ACT_NONE, residual=None, out_dtype=to
 def rms_norm(x, gamma, eps, residual=None, h_out=None, out_dtype=torch.float16):
     """y = h * rsqrt(mean(h^2) + eps) * gamma over the rows of h = x + residual; ``x`` [M, D] fp16 / bfloat16 / fp32, ``gamma`` fp32 [D],
     D <= 32768.  ``out_dtype``: a float type, or "fp8" / "fp4" for an ``MxTensor``.  Without a residual returns y; with one (fp32, or x's
-    type) returns (y, h), h in the residual's type and in ``h_out`` if given, which may be the residual itself."""
+    type) returns (y, h), h in the residual's type and in ``h_out`` if given, which may be the residual itself.  M is below 2^26, 2^24 for
+    D over 2048, 2^22 for D over 8192."""
     who = "rms_norm"
     ldx = _mat(x, who, "x")
     M, D = x.shape

@@ -114,7 +114,8 @@ int csam_linear_f32_batched(void* stream, const float* A, long lda, long strideA
  *           16-byte aligned, ldcodes a multiple of 16;
  *   scales  E8M0 bytes, 2^(s - 127), 255 = NaN: block b = columns 32b .. 32b+31 of row r at scales[(b / 4) * scale_stride + r * 4 + b % 4];
  *           4-byte aligned, scale_stride a multiple of 4 and >= 4 * R.
- * R and K are at most 2^31 - 256.
+ * R and K are at most 2^31 - 256.  Every call of these entries is one launch; calls of 2^32 work items and more are refused (the norm: 2^26
+ * rows of up to 2048 columns, 2^24 of up to 8192, 2^22 of more).
  * f16 / f32 / bf16 = CSAM_DT_F16 / _F32 / _BF16 in these entries and csam_rotary only. */
 #define CSAM_DT_BF16 2
 #define CSAM_MX_FP4 0
