@@ -194,11 +194,20 @@ int rotary_launch(hipStream_t st, RotaryArgs& p) {
   p.by_pair = recip(p.P);
   const long grid = (long)csam_cdiv(p.T, p.tokens) * p.splits;
   CSAM_REQUIRE(csam_launch_fits(grid, 256), "csam_rotary: %d tokens x %d heads of %d are more than one launch takes", p.T, H, p.hd);
-  // Results beyond the L2s' size are stored past them (16384 tokens x 32 heads of 80, interleaved: 30.6 us, 27.7 so; of 128 with 64 pairs,
-  // half: 53.5, 42.1), unless a run of a head ends inside a 64-byte line, which two stores then fill: those meet in the L2 (of 80 with 40
-  // pairs, half: past the caches 61.8, 32.2 so).
-  const bool lines = !HALF || (p.P * sizeof(T) % 64 == 0 && rest * sizeof(T) % 64 == 0);
-  const bool past = lines && (long)p.T * H * p.hd * (long)sizeof(T) > (32L << 20);
+  // Results beyond the L2s' size that do not overwrite their input are stored past the caches where lines belong to one store each: lines
+  // that two stores fill have to meet in the L2.  us through the caches / past them, fp16:
+  //   half, runs of whole lines of 128 bytes: 16384 tokens x 32 heads of 128 with 64 pairs 49.0 / 42.3; in place 44.7 / 48.9
+  //   the same 16 bytes off the lines: 51.4 / 99.0; runs of 64 bytes (heads of 64 with 32 pairs) 24.3 / 27.2, of 80 (80 with 40) 32.3 / 61.6
+  //   interleaved: a wave's stores are one run over the heads, only its ends share lines: 32 heads of 128 48.3 / 41.6, 6 bytes off the lines
+  //   54.8 / 45.0, of 80 30.3 / 28.6, in place 31.1 / 31.0
+  //   interleaved with pieces, which share a line each: 64 heads of 36 33.6 / 50.3, 32 of 97 46.0 / 49.0, 20 of 250 86.4 / 69.6; fp32: 64
+  //   heads of 34 69.7 / 50.6, 32 of 97 89.6 / 66.5
+  constexpr long LINE = 128;
+  auto whole = [&](const void* to, long ld, long hs) { return (uintptr_t)to % LINE == 0 && ld * sizeof(T) % LINE == 0 && hs * sizeof(T) % LINE == 0; };
+  const bool lines = HALF ? p.P * sizeof(T) % LINE == 0 && rest * sizeof(T) % LINE == 0 && whole(p.qo, p.ldqo, p.hsqo) &&
+                                (!p.Hk || whole(p.ko, p.ldko, p.hsko))
+                          : !pieces || p.hd * (long)sizeof(T) >= LINE;
+  const bool past = lines && p.qo != p.q && (long)p.T * H * p.hd * (long)sizeof(T) > (32L << 20);
   if (pieces && past) {                              // (half layouts of whole lines have no pieces)
     if constexpr (!HALF) rotary_kernel<T, HALF, VW, true, true><<<(unsigned)grid, 256, 0, st>>>(p);
   } else if (pieces) rotary_kernel<T, HALF, VW, true, false><<<(unsigned)grid, 256, 0, st>>>(p);

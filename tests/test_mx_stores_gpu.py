@@ -132,7 +132,7 @@ def test_normed_rows_over_the_caches(cuda, dtype, res, out_dtype, m, d):
 @pytest.mark.parametrize("dtype", DTS)
 @pytest.mark.parametrize("T,Hq,Hk,hd,sections,interleaved", [(4201, 20, 12, 128, (32, 32), False), (4201, 32, 0, 128, (16, 16), False), (8401, 24, 8, 64, (16, 16), True),
                                                             (7001, 16, 16, 80, (12, 14, 14), True), (15001, 24, 8, 36, (9, 8), True),
-                                                            (7001, 16, 16, 80, (20, 20), False)])
+                                                            (7001, 16, 16, 80, (20, 20), False), (6001, 24, 8, 97, (40,), True)])
 def test_rotated_rows_over_the_caches(cuda, dtype, T, Hq, Hk, hd, sections, interleaved):
     from crowdsam_amd import hip
     g = torch.Generator(device=cuda).manual_seed(T)
@@ -155,3 +155,25 @@ def test_rotated_rows_over_the_caches(cuda, dtype, T, Hq, Hk, hd, sections, inte
     hip.rotary(q, k, pos, freq, axis, interleaved=interleaved, q_out=q, k_out=k)                  # in place
     for a, b in zip((q, k), before):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", DTS)
+def test_rotated_rows_into_windows(cuda, dtype, interleaved):
+    """Windows on the lines of 128 bytes and off them, by the column, by the row pitch and by k alone: the same bits, the rest untouched."""
+    from crowdsam_amd import hip
+    T, H, hd = 4201, 16, 128
+    x = torch.randn(T, 2 * H * hd, generator=gen(9)).to(dtype).to(cuda)
+    q, k = (x[:, i * H * hd:(i + 1) * H * hd].unflatten(1, (H, hd)) for i in range(2))
+    freq, axis = hip.rotary_frequencies((32, 32))
+    pos = positions(2, T, torch.int32, hd).to(cuda)
+    want = hip.rotary(q, k, pos, freq, axis, interleaved=interleaved)
+    for width, q_at, k_at in ((2 * H * hd + 128, 64, 64 + H * hd), (2 * H * hd + 128, 3, 3 + H * hd), (2 * H * hd + 7, 0, H * hd),
+                              (2 * H * hd + 128, 0, H * hd + 8)):
+        big = torch.full((T, width), 5.0, dtype=dtype, device=cuda)
+        views = [big[:, at:at + H * hd].unflatten(1, (H, hd)) for at in (q_at, k_at)]
+        hip.rotary(q, k, pos, freq, axis, interleaved=interleaved, q_out=views[0], k_out=views[1])
+        for v, w in zip(views, want):
+            assert torch.equal(v, w)
+            v.fill_(5.0)
+        assert bool((big == 5.0).all())
