@@ -258,9 +258,10 @@ int rms_launch_v(hipStream_t st, const RmsArgs& p) {
 template <typename T, int RK>
 int rms_launch(hipStream_t st, const RmsArgs& p) {
   const long yb = p.y_kind >= RMS_MX ? 1 : p.y_kind == CSAM_DT_F32 ? 4 : 2, hb = RK == 0 ? 0 : RK == 2 ? 4 : (long)sizeof(T);
-  // Results that the last-level cache would not hold go past the caches (65536 x 1280 bfloat16, 336 MB: 115 us, 113 so); smaller ones stay
-  // for their reader (21320 x 1024 fp16 with an fp32 residual to E4M3: 43 us, 39 past the caches, but with the product that reads both 83,
-  // past the caches 88).
+  // Results that the last-level cache would not hold go past the caches, whole lines or not (us through them / past them: 65536 x 1280
+  // bfloat16 with residual 118 / 107, x 1279 168 / 153, x 1284 141 / 129; fp16 with an fp32 residual to E4M3 x 1280 167.5 / 163.7, x 1279
+  // 182 / 175; 40000 x 4100 bfloat16 352 / 345); smaller ones stay for their reader (21320 x 1024 fp16 with an fp32 residual to E4M3: 43 us,
+  // 39 past the caches, but with the product that reads both 83, past the caches 88).
   const bool past = (long)p.M * p.D * (yb + hb) > (256L << 20);
   if constexpr (sizeof(T) == 4 || RK == 2) return past ? rms_launch_v<T, RK, 4, true>(st, p) : rms_launch_v<T, RK, 4, false>(st, p);
   else if (p.y_kind == CSAM_DT_F32) return past ? rms_launch_v<T, RK, 4, true>(st, p) : rms_launch_v<T, RK, 4, false>(st, p);
