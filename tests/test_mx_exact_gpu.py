@@ -144,3 +144,18 @@ def test_the_choice_changes_nothing_for_e2m1(cuda):
         qw = hip.mx_quantize(torch.randn(900, 300, generator=gen(1)).to(cuda), "fp4")
         outs = [hip.mx_gemm(qa, qw, out_dtype=torch.float32, cut=cut) for cut in (None, False, True)]
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("cut", [None, False, True])
+@pytest.mark.parametrize("m,n,k", [(3, 130, 512), (100, 1000, 300), (300, 900, 300), (2100, 2001, 300)])
+def test_nan_codes(cuda, m, n, k, cut):
+    """E4M3's NaN code, which quantisation never writes: its row becomes NaN, the others keep what they were."""
+    from crowdsam_amd import hip
+    qa, qw, _ = fine(m, n, k, m + n)
+    whole = hip.mx_gemm(qa, qw, out_dtype=torch.float32, cut=cut)
+    codes = qa.codes.clone()
+    codes[1, k // 2], codes[m - 1, 3] = 0x7F, 0xFF
+    out = hip.mx_gemm(qa._replace(codes=codes), qw, out_dtype=torch.float32, cut=cut)
+    bad = torch.zeros(m, dtype=torch.bool, device=cuda)
+    bad[1] = bad[m - 1] = True
+    assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], whole[~bad])
