@@ -688,9 +688,10 @@ int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
   return CSAM_OK;
 }
 
-// Which form.  The products are bound by moving their operands from L2 to LDS (7 to 9 TB/s beside the matrix units) and by the clock that
-// the matrix units' power leaves: the largest tile wins that fills the chip, and where K is short, one that leaves room for a second
-// workgroup per CU, whose main loop covers the first one's epilogue.  us, fp16 out, each pair measured on one MI355X:
+// Which form.  The tiles move their operands from L2 to LDS at 6 to 9 TB/s while the matrix pipes are busy a third to a half of the time, at
+// the clock that their power leaves: the largest tile wins that fills the chip, and where K is short, one that leaves room for a second
+// workgroup per CU, whose main loop covers the first one's epilogue.  GELU makes the epilogue longer, so with it "short" goes further.
+// us, fp16 out, each pair measured on one MI355X:
 //   M x N x K              E2M1                                       E4M3
 //   32 x 4096 x 4096       rows 5.7, 64x64 6.7                        rows 7.5, 64x64 7.8
 //   224 x 4096 x 4096      64x64 7.8 (three stages 8.2), 128x64 10.2  64x64 9.2 (three stages 10.9), 64x128 11.4
@@ -699,9 +700,12 @@ int mx_tiles(hipStream_t st, const MxGemmArgs& p) {
 //   2048 x 4096 x 4096     64x64 34.7, 128x128 26.2, 256x256 32.6     64x64 50.6, 128x256 32.0, 256x256 45.9
 //   2048 x 4096 x 1024     64x64 17.6, 128x128 13.6, 256x256 15.9     64x64 19.8, 128x256 14.6, 128x128 16.2
 //   4096 x 4096 x 1024     256x256 22.8, 128x128 24.7                 256x256 25.0, 128x128 27.8
-//   5330 x 4096 x 1024     128x128 29.7 (256-wide steps 31.4)         128x128 36.7, 256x256 41.8
-//     with GELU            128x128 35.5 (256-wide steps 39.5)         128x128 40.3, 128x256 45.2
-//   21320 x 4096 x 1024    128x128 104, 256x256 119, with GELU 126, 169    133, 141, with GELU 165, 180
+//   5330 x 4096 x 1024     128x128 29.3 (256-wide steps 31.5)         128x128 33.4, 128x256 34.3, 256x256 37.9
+//     with GELU            128x128 33.0 (256-wide steps 37.5)         128x128 38.6, 128x256 41.7, 256x256 47.6
+//   21320 x 4096 x 1024    128x128 92, 256x256 93, with GELU 106, 127     109, 113, with GELU 127, 145
+//   16384 x 5120 x 1280    128x128 102, 256x256 91, with GELU 114, 121    120, 113, with GELU 135, 139
+//   33000 x 4096 x 1792    128x128 201, 256x256 194, with GELU 223, 244   238, 247, with GELU 265, 290
+//   8192 x 4096 x 2048     128x128 57.7, 256x256 51.5, with GELU 64.6, 61.3    69.1, 66.2, with GELU 77.5, 75.2
 //   5330 x 4096 x 4096     128x128 68.2 (128-wide steps 76.7), 256x256 72.5    128x256 87.1, 128x128 97.8, 256x256 98.5
 //   16384 x 4096 x 4096    128x128 218, 256x256 183                   128x256 292, 256x256 267
 template <int FA>
@@ -721,7 +725,7 @@ int mx_gemm_launch(hipStream_t st, const MxGemmArgs& p) {
   }
   if (few) return mx_rows<FA, false>(st, p, t16);
   const long t256 = (long)csam_cdiv(p.M, 256) * csam_cdiv(p.N, 256), rounds = (t256 + 255) / 256;
-  const bool brief = p.Kp <= 1024;
+  const bool brief = p.Kp <= (p.act == CSAM_ACT_GELU ? 1792 : 1024);
   const bool large = brief ? t256 >= 240 && rounds == 1 : rounds >= 4 || t256 * 4 >= rounds * 256 * 3;
   if constexpr (FA == CSAM_MX_FP4) {
     const long t128 = (long)csam_cdiv(p.M, 128) * csam_cdiv(p.N, 128);
