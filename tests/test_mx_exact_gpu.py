@@ -159,3 +159,14 @@ def test_nan_codes(cuda, m, n, k, cut):
     bad = torch.zeros(m, dtype=torch.bool, device=cuda)
     bad[1] = bad[m - 1] = True
     assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], whole[~bad])
+
+
+@pytest.mark.parametrize("at", [(-59, -59), (-62, -70), (-118, 0), (0, -118)])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_products_below_the_normal_range(cuda, at, m, n, k):
+    """Sums of normal size of products that are subnormal: multiples of 2^-10 times 2^-118 or 2^-132, which fp32 holds."""
+    from crowdsam_amd import hip
+    qa, qw, ref = fine(m, n, k, m + n + 3)
+    groups = qa.scales.shape[0]
+    out = hip.mx_gemm(scaled(qa, [at[0]] * groups), scaled(qw, [at[1]] * groups), out_dtype=torch.float32)
+    assert torch.equal(out.cpu().double(), ref * 2.0 ** sum(at))
